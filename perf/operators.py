@@ -215,10 +215,10 @@ def _plain_int8(state):
     case, x = state["case"], state["x"].float()
     dim = -1 if case["layout"] == "rows" else 1
     most = x.abs().amax(dim, keepdim=True).clamp_min(_TINY)
-    q = (x * (127.0 / most)).round()
+    q = (x * torch.div(torch.full_like(most, 127.0), most)).round()  # a number over a tensor would be its reciprocal, rounded twice
     w = state["weight"].float()
     acc = q @ w.t() if dim == -1 else w @ q
-    y = acc * (most / 127.0) * _wide(case, state["scale"]) + _wide(case, state["bias"])
+    y = acc * torch.div(most, torch.full_like(most, 127.0)) * _wide(case, state["scale"]) + _wide(case, state["bias"])
     return {"y": y.to(state["x"].dtype)}
 
 
