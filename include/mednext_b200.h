@@ -310,6 +310,60 @@ int mednext_ce_bwd(const void* logits, const int64_t* target, const float* fwd_o
                    const float* grad_loss, void* grad, int64_t n, int64_t k, int64_t v,
                    int64_t ignore_index, int dtype, mednext_stream_t stream);
 
+/* ---------------- layer norm over one axis --------------------------------
+ * x, y: contiguous [outer, c, inner], normalised over c (inner = 1: rows of a
+ * [tokens, c] matrix; inner > 1: the channels of each voxel of an NCDHW tensor):
+ *   y = (x - mean) r weight + bias, r = (var + eps)^-1/2, var about the mean / c.
+ * FLOAT32, BFLOAT16 or FLOAT16; weight / bias [c] in param_dtype (FLOAT32 or dtype),
+ * NULL = ones / zeros.  stats: FLOAT32 [outer*inner][2] = (mean, r) for the backward,
+ * or NULL.  fp32 arithmetic, one rounding.  No tokens (outer or inner 0) is no work.
+ * c <= 2^24, outer*c*inner <= 2^40.  No reference counterpart. */
+int mednext_ln_fwd(const void* x, const void* weight, const void* bias, void* y, float* stats,
+                   int64_t outer, int64_t c, int64_t inner, float eps, int dtype, int param_dtype,
+                   mednext_stream_t stream);
+/* dx (dtype) and dweight, dbias (param_dtype, [c], either NULL: not wanted) from dy.
+ * workspace: mednext_ln_bwd_workspace_size bytes, 16-byte aligned; needed when dweight
+ * or dbias is.  Deterministic.  With no tokens dweight and dbias are zeros. */
+size_t mednext_ln_bwd_workspace_size(int64_t outer, int64_t c, int64_t inner, int dtype);
+int mednext_ln_bwd(const void* dy, const void* x, const float* stats, const void* weight, void* dx,
+                   void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
+                   int64_t outer, int64_t c, int64_t inner, int dtype, int param_dtype,
+                   mednext_stream_t stream);
+
+/* ---------------- dropout from a counter-based generator -------------------
+ * y[i] = residual[i] + (word(i) >= drop ? x[i] * 65536 / (65536 - drop) : 0), i < n,
+ * residual NULL = 0; word(i): 16-bit word i % 8 of Philox4x32-10 at counter
+ * (i / 8, offset), key seed.  drop = 65536 * rate, 0..65536.  The mask is not stored:
+ * the backward is the same call on dy with the same seed and offset.  rng: device
+ * int64 {seed, offset}, added to the two arguments (modulo 2^64) when the kernel runs,
+ * so that a captured graph follows it, or NULL.  used: device int64[2] that receives the
+ * pair this call used, or NULL.  A dropped element is 0 whatever x holds.  FLOAT32, BFLOAT16 or
+ * FLOAT16, fp32 arithmetic, one rounding.  y may be x.  No reference counterpart. */
+int mednext_dropout(const void* x, const void* residual, void* y, const int64_t* rng,
+                    uint64_t seed, uint64_t offset, int64_t* used, int64_t n, int drop, int dtype,
+                    mednext_stream_t stream);
+
+/* ---------------- products in 8-bit integers -------------------------------
+ * quantize: x [outer, k, inner] (FLOAT32, BFLOAT16 or FLOAT16) to one 8-bit row per
+ * token, q [outer*inner][q_pitch] (columns k..q_pitch-1 zero; q 16-byte aligned,
+ * q_pitch a multiple of 16), and scale [outer*inner] (FLOAT32):
+ *   m = max(max |x|, 127 * 2^-126), scale = m / 127, q = rint(x * (127 / m)).
+ * A token that holds an infinity or a NaN gets q = 0 and that scale.  Weights are
+ * quantised the same way, a row per output channel.  k <= 131072, outer*inner <= 2^30. */
+int mednext_int8_quantize(const void* x, int8_t* q, float* scale, int64_t outer, int64_t k,
+                          int64_t inner, int64_t q_pitch, int dtype, mednext_stream_t stream);
+/* y [outer, n, inner] = scale_t * weight_scale[j] * sum_k q[t, k] weight[j, k] + bias[j]
+ * with q, scale of x as above; weight: 8-bit [n][weight_pitch], 16-byte aligned,
+ * weight_pitch a multiple of 16 (columns past k are not used); weight_scale [n], bias
+ * [n] or NULL (FLOAT32); y in x's type.  The integer sum is exact, the rest fp32 with
+ * one rounding.  No reference counterpart. */
+size_t mednext_int8_linear_workspace_size(int64_t outer, int64_t k, int64_t inner, int64_t n,
+                                          int dtype);
+int mednext_int8_linear(const void* x, const int8_t* weight, const float* weight_scale,
+                        const float* bias, void* y, void* workspace, size_t workspace_bytes,
+                        int64_t outer, int64_t k, int64_t inner, int64_t n, int64_t weight_pitch,
+                        int dtype, mednext_stream_t stream);
+
 /* ---------------- pointwise 1x1x1 convolution (tensor cores) -------------
  * Forward / input-grad form, one GEMM per sample with the voxel axis as M:
  *   y[s, j, v] = epi( sum_k wt[j, k] * pro(a[s, k, v]) )     j < cout, k < cin

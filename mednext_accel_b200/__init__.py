@@ -14,6 +14,7 @@ from .adaptive import (
     ModelOptimizationContext,
     install_adaptive_operators,
 )
+from .drop import dropout
 from .grn import (
     AdaptiveGlobalResponseNorm3d,
     GlobalResponseNorm3d,
@@ -36,6 +37,7 @@ from .network import (
     mednext_medium,
     mednext_small,
 )
+from .norm import LayerNorm3d, layer_norm
 from .optimization import (
     ExecutionContext,
     ImplementationRegistry,
@@ -46,6 +48,7 @@ from .optimization import (
     PolicyResolver,
     default_implementation_registry,
 )
+from .quant import Int8Pointwise3d, int8_linear, quantize_int8
 
 __version__ = "0.1.0"
 
@@ -61,6 +64,8 @@ __all__ = [
     "ExecutionContext",
     "ImplementationRegistry",
     "ImplementationSpec",
+    "Int8Pointwise3d",
+    "LayerNorm3d",
     "MedNeXtBlock",
     "MedNeXtDownBlock",
     "MedNeXtUpBlock",
@@ -74,10 +79,14 @@ __all__ = [
     "PolicyResolver",
     "cross_entropy",
     "default_implementation_registry",
+    "dropout",
     "get_mednext_v1_config",
     "install_adaptive_operators",
+    "int8_linear",
+    "layer_norm",
     "mednext_base",
     "mednext_large",
     "mednext_medium",
     "mednext_small",
+    "quantize_int8",
 ]

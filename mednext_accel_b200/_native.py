@@ -17,6 +17,7 @@ import os
 from pathlib import Path
 
 import torch
+from torch import Tensor
 
 LIB_NAME = "libmednext_b200.so"
 LIB_PATH = Path(__file__).resolve().parent / "lib" / LIB_NAME
@@ -55,6 +56,7 @@ _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 _SZ = ctypes.c_size_t
 _F = ctypes.c_float
+_U64 = ctypes.c_uint64
 _DIMS5 = [_I64] * 5
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mednext_abi_version": (_INT, []),
@@ -128,6 +130,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mednext_grn_workspace_size": (_SZ, [_I64, _I64, _I64, _INT]),
     "mednext_grn_fwd": (_INT, [_P, _P, _P, _P, _P, _P, _P, _SZ, _I64, _I64, _I64, _F, _INT, _P]),
     "mednext_grn_bwd": (_INT, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _I64, _I64, _I64, _INT, _P]),
+    "mednext_ln_fwd": (_INT, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _F, _INT, _INT, _P]),
+    "mednext_ln_bwd_workspace_size": (_SZ, [_I64, _I64, _I64, _INT]),
+    "mednext_ln_bwd": (_INT, [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _I64, _I64, _I64, _INT, _INT, _P]),
+    "mednext_dropout": (_INT, [_P, _P, _P, _P, _U64, _U64, _P, _I64, _INT, _INT, _P]),
+    "mednext_int8_quantize": (_INT, [_P, _P, _P, _I64, _I64, _I64, _I64, _INT, _P]),
+    "mednext_int8_linear_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _INT]),
+    "mednext_int8_linear": (_INT, [_P, _P, _P, _P, _P, _P, _SZ, _I64, _I64, _I64, _I64, _I64, _INT, _P]),
     "mednext_gn_bwd_from_partials": (
         _INT,
         [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _INT, _INT, _INT, _INT, _P],
@@ -215,6 +224,20 @@ def require_device(t: torch.Tensor) -> None:
     with torch.cuda.device(index):
         check(load().mednext_check_device(), "mednext_check_device")
     _device_checked.add(index)
+
+
+def launch(name: str, t: Tensor, *args) -> None:
+    """Call entry point ``name`` with ``args`` and the current stream of ``t``'s device,
+    that device being current (it need not be the caller's), and check its status."""
+    index = t.get_device()
+    fn = getattr(load(), name)
+    if index == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != OK:
+        check(status, name)
 
 
 def device_error() -> int:
