@@ -331,7 +331,7 @@ int mednext_ln_bwd(const void* dy, const void* x, const float* stats, const void
                    mednext_stream_t stream);
 
 /* ---------------- dropout from a counter-based generator -------------------
- * y[i] = residual[i] + (word(i) >= drop ? x[i] * 65536 / (65536 - drop) : 0), i < n,
+ * y[i] = residual[i] + (word(i) >= drop ? x[i] * 65536 / (65536 - drop) : 0), i < n <= 2^40,
  * residual NULL = 0; word(i): 16-bit word i % 8 of Philox4x32-10 at counter
  * (i / 8, offset), key seed.  drop = 65536 * rate, 0..65536.  The mask is not stored:
  * the backward is the same call on dy with the same seed and offset.  rng: device

@@ -26,28 +26,55 @@ struct DropArgs {
   float scale;
 };
 
-__device__ __forceinline__ uint4 philox4x32_10(uint64_t ctr_lo, uint64_t ctr_hi, uint64_t key) {
-  uint32_t a = (uint32_t)ctr_lo, b = (uint32_t)(ctr_lo >> 32), c = (uint32_t)ctr_hi, d = (uint32_t)(ctr_hi >> 32);
+// The words of U groups, a block's worth of threads apart: counters (hi, lo + u * threads).
+// The rounds run side by side, so that each round key is made once.  `hi`, the offset and the
+// keys are the same in every thread of the CTA: the first products of them are too.
+template <int U>
+__device__ __forceinline__ void philox4x32_10(uint32_t lo, uint32_t hi, uint64_t offset, uint64_t key,
+                                              uint32_t (&w)[U][4]) {
   uint32_t k0 = (uint32_t)key, k1 = (uint32_t)(key >> 32);
 #pragma unroll
+  for (int u = 0; u < U; ++u) {
+    w[u][0] = lo + u * kDropThreads;
+    w[u][1] = hi;
+    w[u][2] = (uint32_t)offset;
+    w[u][3] = (uint32_t)(offset >> 32);
+  }
+#pragma unroll
   for (int i = 0; i < 10; ++i) {
-    const uint64_t p = (uint64_t)0xD2511F53u * a, q = (uint64_t)0xCD9E8D57u * c;
-    a = (uint32_t)(q >> 32) ^ b ^ k0;
-    b = (uint32_t)q;
-    c = (uint32_t)(p >> 32) ^ d ^ k1;
-    d = (uint32_t)p;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint64_t p = (uint64_t)0xD2511F53u * w[u][0], q = (uint64_t)0xCD9E8D57u * w[u][2];
+      w[u][0] = (uint32_t)(q >> 32) ^ w[u][1] ^ k0;
+      w[u][1] = (uint32_t)q;
+      w[u][2] = (uint32_t)(p >> 32) ^ w[u][3] ^ k1;
+      w[u][3] = (uint32_t)p;
+    }
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
-  return make_uint4(a, b, c, d);
 }
 
-// A dropped element gives 0 whatever x holds there (infinities and NaN included).
-__device__ __forceinline__ float drop_one(uint32_t word, uint32_t drop, float x, float scale) {
-  return word >= drop ? __fmul_rn(x, scale) : 0.f;
-}
+// x scale where the word's low (high) 16 bits reach drop, else 0 whatever x holds
+// (infinities and NaN included).  threshold = drop << 16; none: drop = 65536.
+struct DropRule {
+  uint32_t threshold;
+  bool none;
+  float scale;
+  __device__ __forceinline__ float2 pair(uint32_t word, float2 x) const {
+    const float2 v = __fmul2_rn(x, make_float2(scale, scale));
+    return make_float2((word << 16) >= threshold && !none ? v.x : 0.f, word >= threshold && !none ? v.y : 0.f);
+  }
+};
 
-template <typename T>
+// Eight elements, one generator call, per group; U groups per thread, their loads issued
+// before the generator runs.  VEC: every tensor starts on 16 bytes, and CTAs whose groups
+// are all whole move 16-byte vectors; RES: a residual is added.  One turn per CTA.
+//
+// Bound by instructions, not by bytes: about 5 per element for the generator (4 a round)
+// and 5 for the rest against 4 or 6 bytes of traffic.  U = 4 over 2 shares the round keys
+// and keeps 64 bytes of x in flight per thread.
+template <typename T, bool VEC, bool RES, int U>
 __global__ void __launch_bounds__(kDropThreads) dropout_kernel(DropArgs a) {
   uint64_t seed = a.seed, offset = a.offset;
   if (a.rng != nullptr) {
@@ -58,30 +85,79 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(DropArgs a) {
     a.used[0] = (int64_t)seed;
     a.used[1] = (int64_t)offset;
   }
-  const T* x = static_cast<const T*>(a.x);
-  const T* res = static_cast<const T*>(a.residual);
-  T* y = static_cast<T*>(a.y);
-  const long long groups = (a.n + 7) / 8;
-  for (long long g = (long long)blockIdx.x * kDropThreads + threadIdx.x; g < groups;
-       g += (long long)gridDim.x * kDropThreads) {
-    const uint4 r = philox4x32_10((uint64_t)g, offset, seed);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+  const DropRule rule{a.drop << 16, a.drop == 65536u, a.scale};
+  constexpr int kVecs = (int)sizeof(T) / 2;  // vectors per group
+  constexpr int kPer = 8 / kVecs;            // elements per vector
+  constexpr uint32_t kGroups = kDropThreads * U;  // per CTA; a power of two
+  // the CTA's first group: a multiple of kGroups, so that no thread's low word carries
+  const uint64_t g0 = (uint64_t)blockIdx.x * kGroups;
+  const uint32_t lo = (uint32_t)g0 + threadIdx.x, hi = (uint32_t)(g0 >> 32);
+  const long long first = (long long)(g0 + threadIdx.x) * 8;
+  const T* x = static_cast<const T*>(a.x) + first;
+  const T* res = static_cast<const T*>(a.residual) + first;
+  T* y = static_cast<T*>(a.y) + first;
+  uint32_t w[U][4];
+  if (VEC && (long long)(g0 + kGroups) * 8 <= a.n) {
+    uint4 qx[U][kVecs], qr[U][kVecs];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        qx[u][v] = reinterpret_cast<const uint4*>(x + u * kDropThreads * 8)[v];
+        if (RES) qr[u][v] = reinterpret_cast<const uint4*>(res + u * kDropThreads * 8)[v];
+      }
+    philox4x32_10<U>(lo, hi, offset, seed, w);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        float f[kPer], add[kPer];
+        unpack16<T>(qx[u][v], f);
+        if (RES) unpack16<T>(qr[u][v], add);
+#pragma unroll
+        for (int i = 0; i < kPer; i += 2) {
+          float2 t = rule.pair(w[u][(v * kPer + i) / 2], make_float2(f[i], f[i + 1]));
+          if (RES) t = __fadd2_rn(make_float2(add[i], add[i + 1]), t);
+          f[i] = t.x;
+          f[i + 1] = t.y;
+        }
+        reinterpret_cast<uint4*>(y + u * kDropThreads * 8)[v] = pack16<T>(f);
+      }
+    return;
+  }
+  philox4x32_10<U>(lo, hi, offset, seed, w);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const long long i = g * 8 + j;
-      if (i >= a.n) break;
-      const uint32_t word = (j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu;
-      const float v = drop_one(word, a.drop, to_acc<T>(x[i]), a.scale);
-      y[i] = from_acc<T>(res != nullptr ? to_acc<T>(res[i]) + v : v);
+      const int at = u * kDropThreads * 8 + j;
+      if (first + at >= a.n) continue;
+      const float f = to_acc<T>(x[at]);
+      const float2 t = rule.pair(w[u][j >> 1], make_float2(f, f));
+      const float v = (j & 1) ? t.y : t.x;
+      y[at] = from_acc<T>(RES ? to_acc<T>(res[at]) + v : v);
     }
-  }
 }
 
+template <typename T, bool VEC, bool RES, int U>
+int launch_dropout_as(const DropArgs& a, cudaStream_t s) {
+  const long long ctas = ((a.n + 7) / 8 + kDropThreads * U - 1) / (kDropThreads * U);
+  dropout_kernel<T, VEC, RES, U><<<(unsigned)ctas, kDropThreads, 0, s>>>(a);
+  return record_launch();
+}
+template <typename T, bool RES>
+int launch_dropout_for(const DropArgs& a, cudaStream_t s) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) |
+                         reinterpret_cast<uintptr_t>(a.residual);
+  constexpr int U = sizeof(T) == 2 ? 4 : 2;  // 64 bytes of x per thread
+  if (bits % 16 != 0) return launch_dropout_as<T, false, RES, 1>(a, s);
+  // one group per thread while that is all the GPU holds at once
+  if (a.n < 148LL * 2048 * 8 * U) return launch_dropout_as<T, true, RES, 1>(a, s);
+  return launch_dropout_as<T, true, RES, U>(a, s);
+}
 template <typename T>
 int launch_dropout(const DropArgs& a, cudaStream_t s) {
-  const long long blocks = ((a.n + 7) / 8 + kDropThreads - 1) / kDropThreads;
-  dropout_kernel<T><<<(unsigned)std::min<long long>(blocks, 148 * 16), kDropThreads, 0, s>>>(a);
-  return record_launch();
+  return a.residual != nullptr ? launch_dropout_for<T, true>(a, s) : launch_dropout_for<T, false>(a, s);
 }
 
 }  // namespace
@@ -92,7 +168,7 @@ using namespace mednext;
 int mednext_dropout(const void* x, const void* residual, void* y, const int64_t* rng, uint64_t seed, uint64_t offset,
                     int64_t* used, int64_t n, int drop, int dtype, mednext_stream_t stream) {
   if (dtype != MEDNEXT_FLOAT32 && dtype != MEDNEXT_BFLOAT16 && dtype != MEDNEXT_FLOAT16) return MEDNEXT_ERR_BAD_DTYPE;
-  if (n < 0 || n > ((int64_t)1 << 48)) return MEDNEXT_ERR_BAD_SHAPE;
+  if (n < 0 || n > ((int64_t)1 << 40)) return MEDNEXT_ERR_BAD_SHAPE;
   if (drop < 0 || drop > 65536) return MEDNEXT_ERR_BAD_VALUE;
   if (n > 0 && (x == nullptr || y == nullptr)) return MEDNEXT_ERR_NULL_POINTER;
   const size_t esz = elem_size(dtype);

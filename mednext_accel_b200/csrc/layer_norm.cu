@@ -881,7 +881,8 @@ int dw_parts(long long tokens) { return (int)std::max(1LL, std::min((long long)k
 
 template <typename T, int VEC, int EPT, int R, int THREADS>
 int launch_rows_fwd_as(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
-  const long long cap = kSms * (long long)(2048 / p.threads);
+  // as many CTAs as the registers of the launch bounds let reside: 768 or 1024 threads
+  const long long cap = kSms * (long long)((R > 1 ? 768 : 1024) / p.threads);
   ln_rows_fwd_kernel<T, VEC, EPT, R, THREADS>
       <<<(unsigned)std::min((p.units + R - 1) / R, cap), p.threads, 0, s>>>(a, p.G);
   return record_launch();
@@ -923,7 +924,7 @@ int launch_chan_fwd_as(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
   const size_t smem = chan_smem(p, a.C);
   const int st = ensure_smem(kern, smem);
   if (st != MEDNEXT_OK) return st;
-  const long long cap = kSms * (long long)std::max(1, 32 / (p.S * p.P));
+  const long long cap = kSms * (long long)std::max(1, 24 / (p.S * p.P));  // resident: 24 warps
   kern<<<(unsigned)std::min(p.units, cap), dim3(32, p.S, p.P), smem, s>>>(a);
   return record_launch();
 }
@@ -972,7 +973,10 @@ template <typename T>
 int ln_bwd(const LnArgs& a, void* dw, void* db, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const LnPlan p = plan_ln<T>(a, true);
-  int st, parts = (int)std::min<long long>(dw_parts(a.tokens), std::max(1LL, p.units));
+  // one CTA per resident slot (the launch bounds leave 512 threads), one partial per CTA
+  const int warps = p.form == kRows ? p.threads / 32 : p.S * p.P;
+  const long long slots = (long long)kSms * std::max(1, 16 / std::max(1, warps));
+  int st, parts = (int)std::min<long long>(std::min<long long>(dw_parts(a.tokens), slots), std::max(1LL, p.units));
   if (p.form == kRows) {
     if (p.ept == 8)
       st = p.vec ? launch_rows_bwd<T, V, 8>(a, p, parts, s) : launch_rows_bwd<T, 1, 8>(a, p, parts, s);
