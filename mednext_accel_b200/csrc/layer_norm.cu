@@ -263,86 +263,176 @@ __global__ void __launch_bounds__(1024) ln_fold_kernel(const float* __restrict__
   }
 }
 
+// ------------------------------ packed arithmetic ------------------------------
+// All of the register kernels below work on pairs (fp32 x 2 instructions) of values that
+// stay packed in their own type until they are used: these kernels are bound by
+// instruction issue as soon as their loads are wide, so an element's instructions count.
+// centered() subtracts a mean from the packed pair itself, by a mixed-precision FMA with 1
+// for the 16-bit types: the same bits as widening and subtracting, without the widening.
+template <typename T>
+struct Pack {  // 16-bit types: two elements per word
+  using Word = uint32_t;
+  static __device__ __forceinline__ float2 value(uint32_t w) { return unpack2<T>(w); }
+  static __device__ __forceinline__ float2 plus(uint32_t w, float2 add) {
+    return make_float2(mix_fma<T>((uint16_t)(w & 0xffffu), one16<T>(), add.x),
+                       mix_fma<T>((uint16_t)(w >> 16), one16<T>(), add.y));
+  }
+  static __device__ __forceinline__ uint32_t make(float2 v) { return pack2<T>(v); }
+};
+template <>
+struct Pack<float> {
+  using Word = float2;
+  static __device__ __forceinline__ float2 value(float2 w) { return w; }
+  static __device__ __forceinline__ float2 plus(float2 w, float2 add) { return __fadd2_rn(w, add); }
+  static __device__ __forceinline__ float2 make(float2 v) { return v; }
+};
+// Two 16-bit elements in a register each, as single-element loads leave them: packing them
+// would wait for each pair before the next load.
+struct Halves {
+  uint16_t a, b;
+};
+template <typename T>
+struct Apart {
+  using Word = Halves;
+  static __device__ __forceinline__ float2 value(Halves w) {
+    return make_float2(to_acc<T>(reinterpret_cast<const T&>(w.a)), to_acc<T>(reinterpret_cast<const T&>(w.b)));
+  }
+  static __device__ __forceinline__ float2 plus(Halves w, float2 add) {
+    return make_float2(mix_fma<T>(w.a, one16<T>(), add.x), mix_fma<T>(w.b, one16<T>(), add.y));
+  }
+};
+template <>
+struct Apart<float> : Pack<float> {};
+template <typename T, bool SINGLE>
+struct PackFor : Pack<T> {};
+template <typename T>
+struct PackFor<T, true> : Apart<T> {};
+
 // Makes the compiler take the packed words as new values: it unpacks them again (one
-// instruction for two bf16) instead of keeping the unpacked copies in registers.
+// instruction for a bf16) instead of keeping the unpacked copies in registers.
 __device__ __forceinline__ void renew(uint32_t& v) { asm volatile("" : "+r"(v)); }
-__device__ __forceinline__ void renew(float& v) {}
-__device__ __forceinline__ void renew(__nv_bfloat16& v) { asm volatile("" : "+h"(reinterpret_cast<uint16_t&>(v))); }
-__device__ __forceinline__ void renew(__half& v) { asm volatile("" : "+h"(reinterpret_cast<uint16_t&>(v))); }
-__device__ __forceinline__ void renew(uint4& q) {
-  renew(q.x);
-  renew(q.y);
-  renew(q.z);
-  renew(q.w);
-}
+__device__ __forceinline__ void renew(float2&) {}
+__device__ __forceinline__ void renew(Halves& v) { asm volatile("" : "+h"(v.a), "+h"(v.b)); }
 
 // ------------------------------ rows held in registers ------------------------------
-// G threads hold a row, EPT elements each, loaded once as 16-byte vectors (VEC elements;
-// VEC = 1 where rows do not start on 16 bytes) that stay packed until they are used.
-// G <= 32 is a power of two and its sums are shuffles; a larger G is whole warps, which
-// add through shared memory, one barrier per sum, R rows' sums at once.
+// G threads hold a row, EPT elements each, in words of VEC elements (16 bytes; 4 bytes or
+// single elements where rows do not start on 16), word v of thread gl beginning at column
+// (v G + gl) VEC.  G <= 32 is a power of two and its sums are shuffles; wider rows take
+// whole warps, which add through shared memory, one barrier per sum, R rows at once.
+// Up to 1024 columns are one warp's: 32 elements per thread cost 10 shuffles for two
+// sums, against two barriers per row for more warps with fewer elements.
 template <typename T, int VEC, int EPT>
 struct RowFrag {
-  static constexpr int kVecs = EPT / VEC;
-  uint4 q[kVecs];
-  // column of element 0 of vector v
-  static __device__ __forceinline__ int col(int v, int gl, int G) { return (v * G + gl) * VEC; }
+  using P = PackFor<T, VEC == 1>;
+  static constexpr int kChunk = VEC == 1 ? 2 : VEC;  // elements handled together
+  static constexpr int kChunks = EPT / kChunk, kPairs = kChunk / 2;
+  typename P::Word w[EPT / 2];
+  static __device__ __forceinline__ int col(int j, int e, int gl, int G) {  // of element e of chunk j
+    return VEC == 1 ? (2 * j + e) * G + gl : (j * G + gl) * VEC + e;
+  }
   __device__ __forceinline__ void load(const T* row, int gl, int G, int C, bool in) {
 #pragma unroll
-    for (int v = 0; v < kVecs; ++v) {
-      const int c = col(v, gl, G);
-      q[v] = in && c < C ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < kChunks; ++j) {
+      if constexpr (VEC == 1) {
+        const int c0 = col(j, 0, gl, G), c1 = col(j, 1, gl, G);
+        const T a = in && c0 < C ? row[c0] : from_acc<T>(0.f), b = in && c1 < C ? row[c1] : from_acc<T>(0.f);
+        if constexpr (sizeof(T) == 4) w[j] = make_float2(a, b);
+        else w[j] = Halves{reinterpret_cast<const uint16_t&>(a), reinterpret_cast<const uint16_t&>(b)};
+      } else {
+        const int c = col(j, 0, gl, G);
+        const bool ok = in && c < C;
+        if constexpr (sizeof(T) * VEC == 16) {
+          const uint4 q = ok ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+          if constexpr (sizeof(T) == 4) {
+            w[2 * j] = make_float2(__uint_as_float(q.x), __uint_as_float(q.y));
+            w[2 * j + 1] = make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
+          } else {
+            w[4 * j] = q.x; w[4 * j + 1] = q.y; w[4 * j + 2] = q.z; w[4 * j + 3] = q.w;
+          }
+        } else {
+          w[j] = ok ? *reinterpret_cast<const uint32_t*>(row + c) : 0u;
+        }
+      }
     }
   }
-  __device__ __forceinline__ void get(int v, float* f) const { unpack16<T>(q[v], f); }
   __device__ __forceinline__ void again() {
 #pragma unroll
-    for (int v = 0; v < kVecs; ++v) renew(q[v]);
+    for (int i = 0; i < EPT / 2; ++i) renew(w[i]);
   }
-  static __device__ __forceinline__ void store(T* row, int c, const float* f) {
-    *reinterpret_cast<uint4*>(row + c) = pack16<T>(f);
-  }
-};
-template <typename T, int EPT>
-struct RowFrag<T, 1, EPT> {
-  static constexpr int kVecs = EPT;
-  T e[EPT];
-  static __device__ __forceinline__ int col(int v, int gl, int G) { return v * G + gl; }
-  __device__ __forceinline__ void load(const T* row, int gl, int G, int C, bool in) {
-#pragma unroll
-    for (int v = 0; v < EPT; ++v) {
-      const int c = v * G + gl;
-      e[v] = in && c < C ? row[c] : from_acc<T>(0.f);
+  // f: the chunk's pairs
+  static __device__ __forceinline__ void store(T* row, int j, int gl, int G, int C, const float2* f) {
+    const int c = col(j, 0, gl, G);
+    if constexpr (VEC == 1) {
+      if (c < C) row[c] = from_acc<T>(f[0].x);
+      if (c + G < C) row[c + G] = from_acc<T>(f[0].y);
+    } else if constexpr (sizeof(T) * VEC == 16) {
+      if (c >= C) return;
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(row + c) = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+      else *reinterpret_cast<uint4*>(row + c) = make_uint4(P::make(f[0]), P::make(f[1]), P::make(f[2]), P::make(f[3]));
+    } else {
+      if (c < C) *reinterpret_cast<uint32_t*>(row + c) = P::make(f[0]);
     }
   }
-  __device__ __forceinline__ void get(int v, float* f) const { f[0] = to_acc<T>(e[v]); }
-  __device__ __forceinline__ void again() {
-#pragma unroll
-    for (int v = 0; v < EPT; ++v) renew(e[v]);
-  }
-  static __device__ __forceinline__ void store(T* row, int c, const float* f) { row[c] = from_acc<T>(f[0]); }
 };
 
-// p + step as a value of its own: the 32 products k * step of an unrolled loop would
-// otherwise be kept over the loop about it, 64 registers.
-template <typename T>
-__device__ __forceinline__ void advance(T*& p, long long step) {
-  p += step;
-  asm volatile("" : "+l"(p));
-}
-
-// Shared-memory loads that stay where they are written: hoisted out of the loop over
-// tiles, a thread's parameters would take 32 or 64 registers.
-__device__ __forceinline__ float2 lds2(const float2* p) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(smem_u32(p)));
-  return v;
-}
-__device__ __forceinline__ float lds1(const float* p) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(smem_u32(p)));
-  return v;
-}
+// A parameter vector for the fragments: in registers up to 16 elements per thread, else in
+// shared memory (EPT * G floats), where 8-element words are split into two planes of
+// four so that the lanes of a 16-byte load lie side by side.
+template <typename T, int VEC, int EPT>
+struct RowParam {
+  using Frag = RowFrag<T, VEC, EPT>;
+  static constexpr bool kRegs = EPT <= 16;
+  float2 r[kRegs ? EPT / 2 : 1];
+  const float* sm;
+  static size_t smem_bytes(int G) { return kRegs ? 0 : (size_t)EPT * G * sizeof(float); }
+  static __device__ __forceinline__ int place(int c, int G) {
+    if constexpr (VEC == 8) return (((c >> 3) / G * 2 + ((c >> 2) & 1)) * G + (c >> 3) % G) * 4 + (c & 3);
+    else return c;
+  }
+  template <typename F>
+  __device__ __forceinline__ void regs(F at, int gl, int G, int C) {
+#pragma unroll
+    for (int i = 0; i < EPT / 2; ++i) {
+      const int j = i / Frag::kPairs, e = i % Frag::kPairs * 2;
+      const int c0 = Frag::col(j, e, gl, G), c1 = Frag::col(j, e + 1, gl, G);
+      r[i] = make_float2(c0 < C ? at(c0) : 0.f, c1 < C ? at(c1) : 0.f);
+    }
+  }
+  // every thread of the CTA calls this; a barrier follows where shared memory is used
+  __device__ __forceinline__ void fill(const void* p, int dtype, float none, float* smem, int gl, int G, int C) {
+    sm = smem;
+    if constexpr (kRegs) {
+      // the type is told apart once, so that the loads of one vector are in flight together
+      if (p == nullptr) regs([=](int) { return none; }, gl, G, C);
+      else if (dtype == MEDNEXT_FLOAT32) regs([=](int c) { return static_cast<const float*>(p)[c]; }, gl, G, C);
+      else regs([=](int c) { return to_acc<T>(static_cast<const T*>(p)[c]); }, gl, G, C);
+    } else {
+      for (int c = threadIdx.x; c < EPT * G; c += blockDim.x)
+        smem[place(c, G)] = c < C ? load_param(p, dtype, c, none) : 0.f;
+    }
+  }
+  __device__ __forceinline__ void get(int j, int gl, int G, float2* f) const {  // the chunk's pairs
+    if constexpr (kRegs) {
+#pragma unroll
+      for (int i = 0; i < Frag::kPairs; ++i) f[i] = r[j * Frag::kPairs + i];
+    } else if constexpr (VEC == 8) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 q = *reinterpret_cast<const float4*>(sm + ((2 * j + h) * G + gl) * 4);
+        f[2 * h] = make_float2(q.x, q.y);
+        f[2 * h + 1] = make_float2(q.z, q.w);
+      }
+    } else if constexpr (VEC == 4) {
+      const float4 q = *reinterpret_cast<const float4*>(sm + (j * G + gl) * 4);
+      f[0] = make_float2(q.x, q.y);
+      f[1] = make_float2(q.z, q.w);
+    } else if constexpr (VEC == 2) {
+      f[0] = *reinterpret_cast<const float2*>(sm + (j * G + gl) * 2);
+    } else {
+      f[0] = make_float2(sm[Frag::col(j, 0, gl, G)], sm[Frag::col(j, 1, gl, G)]);
+    }
+  }
+};
 
 // Sums of N values over the G threads of a group, the same in each; red holds two
 // buffers of N x 32, taken in turn: the barrier of the next sum separates their uses.
@@ -372,26 +462,21 @@ __device__ __forceinline__ void group_sum(float (&v)[N], int G, float* red, int&
   }
 }
 
-template <typename T, int VEC, int EPT, int R, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? (R > 1 ? 3 : 4) : 1) ln_rows_fwd_kernel(LnArgs a, int G) {
+constexpr int kRowThreads = 256;
+
+template <typename T, int VEC, int EPT, int R>
+__global__ void __launch_bounds__(kRowThreads, 3) ln_rows_fwd_kernel(LnArgs a, int G) {
   using Frag = RowFrag<T, VEC, EPT>;
-  constexpr int kVecs = Frag::kVecs;
+  using P = typename Frag::P;
+  extern __shared__ __align__(16) float ln_sm[];
   __shared__ float red[2 * R * 32];
   int turn = 0;
   const int groups = blockDim.x / G, gi = threadIdx.x / G, gl = threadIdx.x - gi * G;
   const float rc = 1.f / (float)a.C;
-  // up to 8 columns: the parameters stay in registers over the rows
-  float w[EPT <= 8 ? EPT : 1], b[EPT <= 8 ? EPT : 1];
-  if (EPT <= 8) {
-#pragma unroll
-    for (int v = 0; v < kVecs; ++v)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int c = Frag::col(v, gl, G) + i;
-        w[(v * VEC + i) % (EPT <= 8 ? EPT : 1)] = c < a.C ? load_param(a.w, a.pdt, c, 1.f) : 0.f;
-        b[(v * VEC + i) % (EPT <= 8 ? EPT : 1)] = c < a.C ? load_param(a.b, a.pdt, c, 0.f) : 0.f;
-      }
-  }
+  RowParam<T, VEC, EPT> w, b;
+  w.fill(a.w, a.pdt, 1.f, ln_sm, gl, G, a.C);
+  b.fill(a.b, a.pdt, 0.f, ln_sm + EPT * G, gl, G, a.C);
+  if (!w.kRegs) __syncthreads();
   for (long long base = (long long)blockIdx.x * groups * R; base < a.tokens; base += (long long)gridDim.x * groups * R) {
     Frag x[R];
     float s[R];
@@ -402,34 +487,32 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? (R > 1 ? 3 : 4) : 1)
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      s[r] = 0.f;
+      float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v) {
-        float f[VEC];
-        x[r].get(v, f);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) s[r] += f[i];
-      }
+      for (int i = 0; i < EPT / 2; ++i) sum = P::plus(x[r].w[i], sum);
+      s[r] = sum.x + sum.y;
     }
     group_sum<R>(s, G, red, turn);
-    float mean[R];
+    float2 nm[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
+      nm[r] = f2(-s[r] * rc);
       x[r].again();
-      mean[r] = s[r] * rc;
-      s[r] = 0.f;
+      float2 sq = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v) {
-        float f[VEC];
-        x[r].get(v, f);
-        if (Frag::col(v, gl, G) < a.C) {
+      for (int j = 0; j < Frag::kChunks; ++j) {
+        if (VEC > 1 && Frag::col(j, 0, gl, G) >= a.C) continue;
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float d = f[i] - mean[r];
-            s[r] = fmaf(d, d, s[r]);
+        for (int i = 0; i < Frag::kPairs; ++i) {
+          float2 d = P::plus(x[r].w[j * Frag::kPairs + i], nm[r]);
+          if (VEC == 1) {
+            if (Frag::col(j, 0, gl, G) >= a.C) d.x = 0.f;
+            if (Frag::col(j, 1, gl, G) >= a.C) d.y = 0.f;
           }
+          sq = __ffma2_rn(d, d, sq);
         }
       }
+      s[r] = sq.x + sq.y;
     }
     group_sum<R>(s, G, red, turn);
 #pragma unroll
@@ -440,45 +523,38 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? (R > 1 ? 3 : 4) : 1)
       const float rstd = rsqrtf(s[r] * rc + a.eps);
       T* y = static_cast<T*>(a.y) + t * a.C;
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v) {
-        const int c = Frag::col(v, gl, G);
-        if (c >= a.C) continue;
-        float f[VEC];
-        x[r].get(v, f);
+      for (int j = 0; j < Frag::kChunks; ++j) {
+        float2 f[Frag::kPairs], pw[Frag::kPairs], pb[Frag::kPairs];
+        w.get(j, gl, G, pw);
+        b.get(j, gl, G, pb);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float wi = EPT <= 8 ? w[(v * VEC + i) % (EPT <= 8 ? EPT : 1)] : load_param(a.w, a.pdt, c + i, 1.f);
-          const float bi = EPT <= 8 ? b[(v * VEC + i) % (EPT <= 8 ? EPT : 1)] : load_param(a.b, a.pdt, c + i, 0.f);
-          f[i] = fmaf((f[i] - mean[r]) * rstd, wi, bi);
-        }
-        Frag::store(y, c, f);
+        for (int i = 0; i < Frag::kPairs; ++i)
+          f[i] = __ffma2_rn(__fmul2_rn(P::plus(x[r].w[j * Frag::kPairs + i], nm[r]), f2(rstd)), pw[i], pb[i]);
+        Frag::store(y, j, gl, G, a.C, f);
       }
-      if (a.stats != nullptr && gl == 0) a.stats[t] = make_float2(mean[r], rstd);
+      if (a.stats != nullptr && gl == 0) a.stats[t] = make_float2(-nm[r].x, rstd);
     }
   }
 }
 
 // The threads own their columns over all rows of the CTA, so the weight grads are sums
-// in registers; the CTA adds its groups' sums through shared memory (acc: [slots][2][C],
-// a slot per warp for G <= 32, per group else) and writes one partial per CTA.
-template <typename T, int VEC, int EPT, int R, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? (R > 1 ? 2 : 3) : 1) ln_rows_bwd_kernel(LnArgs a, int G) {
+// in registers; the CTA adds its groups' sums through shared memory ([slots][2][C], a
+// slot per warp for G <= 32, per group else) and writes one partial per CTA.
+template <typename T, int VEC, int EPT, int R>
+__global__ void __launch_bounds__(kRowThreads, 2) ln_rows_bwd_kernel(LnArgs a, int G) {
   using Frag = RowFrag<T, VEC, EPT>;
-  constexpr int kVecs = Frag::kVecs;
-  extern __shared__ __align__(16) float ln_acc[];
+  using P = typename Frag::P;
+  extern __shared__ __align__(16) float ln_sm[];
   __shared__ float red[2 * 2 * R * 32];
   int turn = 0;
   const int groups = blockDim.x / G, gi = threadIdx.x / G, gl = threadIdx.x - gi * G;
   const float rc = 1.f / (float)a.C;
-  float w[EPT], dw[EPT], db[EPT];
+  RowParam<T, VEC, EPT> w;
+  w.fill(a.w, a.pdt, 1.f, ln_sm, gl, G, a.C);
+  if (!w.kRegs) __syncthreads();
+  float2 dw[EPT / 2], db[EPT / 2];
 #pragma unroll
-  for (int v = 0; v < kVecs; ++v)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const int c = Frag::col(v, gl, G) + i;
-      w[v * VEC + i] = c < a.C ? load_param(a.w, a.pdt, c, 1.f) : 0.f;
-      dw[v * VEC + i] = db[v * VEC + i] = 0.f;
-    }
+  for (int i = 0; i < EPT / 2; ++i) dw[i] = db[i] = make_float2(0.f, 0.f);
   for (long long base = (long long)blockIdx.x * groups * R; base < a.tokens; base += (long long)gridDim.x * groups * R) {
     Frag x[R], d[R];
     float2 st[R];
@@ -493,21 +569,24 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? (R > 1 ? 2 : 3) : 1)
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      s[2 * r] = s[2 * r + 1] = 0.f;
+      float2 s1 = make_float2(0.f, 0.f), s2 = s1;
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v) {
-        float f[VEC], g[VEC];
-        x[r].get(v, f);
-        d[r].get(v, g);
+      for (int j = 0; j < Frag::kChunks; ++j) {
+        float2 pw[Frag::kPairs];
+        w.get(j, gl, G, pw);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float xh = (f[i] - st[r].x) * st[r].y, gw = g[i] * w[v * VEC + i];
-          dw[v * VEC + i] = fmaf(g[i], xh, dw[v * VEC + i]);
-          db[v * VEC + i] += g[i];
-          s[2 * r] += gw;
-          s[2 * r + 1] = fmaf(gw, xh, s[2 * r + 1]);
+        for (int i = 0; i < Frag::kPairs; ++i) {
+          const int n = j * Frag::kPairs + i;
+          const float2 xh = __fmul2_rn(P::plus(x[r].w[n], f2(-st[r].x)), f2(st[r].y));
+          const float2 g = P::value(d[r].w[n]), gw = __fmul2_rn(g, pw[i]);
+          dw[n] = __ffma2_rn(g, xh, dw[n]);
+          db[n] = __fadd2_rn(db[n], g);
+          s1 = __fadd2_rn(s1, gw);
+          s2 = __ffma2_rn(gw, xh, s2);
         }
       }
+      s[2 * r] = s1.x + s1.y;
+      s[2 * r + 1] = s2.x + s2.y;
     }
     group_sum<2 * R>(s, G, red, turn);
 #pragma unroll
@@ -516,182 +595,278 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? (R > 1 ? 2 : 3) : 1)
       if (t >= a.tokens) continue;
       x[r].again();
       d[r].again();
-      const float m1 = s[2 * r] * rc, m2 = s[2 * r + 1] * rc;
+      const float2 m1 = f2(-s[2 * r] * rc), m2 = f2(-s[2 * r + 1] * rc);
       T* dx = static_cast<T*>(a.y) + t * a.C;
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v) {
-        const int c = Frag::col(v, gl, G);
-        if (c >= a.C) continue;
-        float f[VEC], g[VEC];
-        x[r].get(v, f);
-        d[r].get(v, g);
+      for (int j = 0; j < Frag::kChunks; ++j) {
+        float2 f[Frag::kPairs], pw[Frag::kPairs];
+        w.get(j, gl, G, pw);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float xh = (f[i] - st[r].x) * st[r].y;
-          f[i] = st[r].y * (fmaf(g[i], w[v * VEC + i], -m1) - xh * m2);
+        for (int i = 0; i < Frag::kPairs; ++i) {
+          const int n = j * Frag::kPairs + i;
+          const float2 xh = __fmul2_rn(P::plus(x[r].w[n], f2(-st[r].x)), f2(st[r].y));
+          const float2 t1 = __ffma2_rn(P::value(d[r].w[n]), pw[i], m1);
+          f[i] = __fmul2_rn(__ffma2_rn(xh, m2, t1), f2(st[r].y));
         }
-        Frag::store(dx, c, f);
+        Frag::store(dx, j, gl, G, a.C, f);
       }
     }
   }
   if (a.part == nullptr) return;
   // lanes of one warp that hold the same columns, then the CTA's slots, in order
 #pragma unroll
-  for (int i = 0; i < EPT; ++i)
+  for (int i = 0; i < EPT / 2; ++i)
     for (int o = G; o < 32; o <<= 1) {
-      dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
-      db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
+      dw[i].x += __shfl_xor_sync(0xffffffffu, dw[i].x, o);
+      dw[i].y += __shfl_xor_sync(0xffffffffu, dw[i].y, o);
+      db[i].x += __shfl_xor_sync(0xffffffffu, db[i].x, o);
+      db[i].y += __shfl_xor_sync(0xffffffffu, db[i].y, o);
     }
+  __syncthreads();  // the parameters in shared memory give way
   const int slot = G < 32 ? threadIdx.x >> 5 : gi, slots = G < 32 ? blockDim.x >> 5 : groups;
   if (G >= 32 || (threadIdx.x & 31) < G) {
 #pragma unroll
-    for (int v = 0; v < kVecs; ++v)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int c = Frag::col(v, gl, G) + i;
-        if (c < a.C) {
-          ln_acc[(size_t)(2 * slot) * a.C + c] = dw[v * VEC + i];
-          ln_acc[(size_t)(2 * slot + 1) * a.C + c] = db[v * VEC + i];
-        }
+    for (int i = 0; i < EPT / 2; ++i) {
+      const int j = i / Frag::kPairs, e = i % Frag::kPairs * 2;
+      const int c0 = Frag::col(j, e, gl, G), c1 = Frag::col(j, e + 1, gl, G);
+      float* at = ln_sm + (size_t)(2 * slot) * a.C;
+      if (c0 < a.C) {
+        at[c0] = dw[i].x;
+        at[a.C + c0] = db[i].x;
       }
+      if (c1 < a.C) {
+        at[c1] = dw[i].y;
+        at[a.C + c1] = db[i].y;
+      }
+    }
   }
   __syncthreads();
   for (int c = threadIdx.x; c < 2 * a.C; c += blockDim.x) {
     float v = 0.f;
-    for (int i = 0; i < slots; ++i) v += ln_acc[(size_t)i * 2 * a.C + c];
+    for (int i = 0; i < slots; ++i) v += ln_sm[(size_t)i * 2 * a.C + c];
     a.part[(long long)blockIdx.x * 2 * a.C + c] = v;
   }
 }
 
 // ------------------------------ channels first, held in registers ------------------------------
-// A lane owns W neighbouring tokens (one 32-bit word of 16-bit data, W = 2, where rows
-// start on words and inner is even; else one element) and CPT channels of them; a tile of
-// 32 W tokens takes S = ceil(C / CPT) warps, channel k S + s belonging to warp s.  Each
-// load is one coalesced row segment of a channel, and x is read once.  Only two numbers per token cross the
+// A lane owns W neighbouring tokens and CPT channels of them; a tile of 32 W tokens takes
+// S = ceil(C / CPT) warps, channel k S + s belonging to warp s.  Each load is one coalesced
+// segment of a channel's row, and x is read once.  Only two numbers per token cross the
 // warps, once per tile.  blockDim = (32, S, P), P tiles per CTA side by side.
+//
+// W = 4 (8 bytes of 16-bit data) and W = 2 need inner to be a multiple of W and the tensors
+// to start on a word; W = 1 takes the rest (odd volumes).  The wider word spends 64-bit
+// addresses, parameter loads and predicates on more elements.
+//
+// A slot is what is computed together: one channel of W tokens (pairs of tokens), or, for
+// W = 1, two channels of one token (a pair of channels).
 template <typename T, int W>
-struct Word;
-template <typename T>
-struct Word<T, 1> {
-  T v;
-  __device__ __forceinline__ void load(const T* p, bool in) { v = in ? *p : from_acc<T>(0.f); }
-  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_acc<T>(v); }
-  static __device__ __forceinline__ void store(T* p, const float (&f)[1]) { *p = from_acc<T>(f[0]); }
-};
-template <typename T>
-struct Word<T, 2> {
-  uint32_t v;
-  __device__ __forceinline__ void load(const T* p, bool in) { v = in ? *reinterpret_cast<const uint32_t*>(p) : 0u; }
-  __device__ __forceinline__ void get(float (&f)[2]) const {
-    const float2 t = unpack2<T>(v);
-    f[0] = t.x;
-    f[1] = t.y;
+struct TokenWord {
+  using P = PackFor<T, W == 1>;
+  static constexpr int kPairs = (W + 1) / 2;    // pairs per slot
+  static constexpr int kChans = W == 1 ? 2 : 1;  // channels per slot
+  typename P::Word w[kPairs];
+  // p: the slot's first channel; n: how many of its channels there are; step to the next one
+  __device__ __forceinline__ void load(const T* p, int n, long long step) {
+    if constexpr (W == 1) {
+      const T a = n > 0 ? *p : from_acc<T>(0.f), b = n > 1 ? p[step] : from_acc<T>(0.f);
+      if constexpr (sizeof(T) == 4) w[0] = make_float2(a, b);
+      else w[0] = Halves{reinterpret_cast<const uint16_t&>(a), reinterpret_cast<const uint16_t&>(b)};
+    } else if constexpr (sizeof(T) == 4) {
+      w[0] = n > 0 ? *reinterpret_cast<const float2*>(p) : make_float2(0.f, 0.f);
+    } else if constexpr (W == 4) {
+      const uint2 q = n > 0 ? *reinterpret_cast<const uint2*>(p) : make_uint2(0u, 0u);
+      w[0] = q.x;
+      w[1] = q.y;
+    } else {
+      w[0] = n > 0 ? *reinterpret_cast<const uint32_t*>(p) : 0u;
+    }
   }
-  static __device__ __forceinline__ void store(T* p, const float (&f)[2]) {
-    *reinterpret_cast<uint32_t*>(p) = pack2<T>(make_float2(f[0], f[1]));
+  __device__ __forceinline__ void again() {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) renew(w[i]);
+  }
+  static __device__ __forceinline__ void store(T* p, int n, long long step, const float2* f) {
+    if constexpr (W == 1) {
+      *p = from_acc<T>(f[0].x);
+      if (n > 1) p[step] = from_acc<T>(f[0].y);
+    } else if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float2*>(p) = f[0];
+    } else if constexpr (W == 4) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(P::make(f[0]), P::make(f[1]));
+    } else {
+      *reinterpret_cast<uint32_t*>(p) = P::make(f[0]);
+    }
   }
 };
 
-constexpr int kChanCpt = 32;
+// Channels per thread: 32 registers of packed x.
+template <typename T, int W>
+constexpr int chan_cpt() {
+  return W * (int)sizeof(T) == 8 ? 16 : 32;
+}
+
+// p + step as a value of its own: the products k * step of an unrolled loop would
+// otherwise be kept over the loop about it, 64 registers.
+template <typename T>
+__device__ __forceinline__ void advance(T*& p, long long step) {
+  p += step;
+  asm volatile("" : "+l"(p));
+}
+
+// Shared-memory loads that stay where they are written: hoisted out of the loop over
+// tiles, a thread's parameters would take its registers.
+__device__ __forceinline__ float4 lds4(const float4* p) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(smem_u32(p)));
+  return v;
+}
+__device__ __forceinline__ float2 lds2(const float2* p) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(smem_u32(p)));
+  return v;
+}
+
+// Joins S warps' (x, y) pairs per token through shared memory: join(token's S pairs)
+// runs in one thread per token, spread over the warps, and every thread reads the results of
+// its W tokens.  red: [S][W][32] pairs, then [W][32] results; the first barrier of the
+// next use separates reading these results from writing those.
+template <int W, typename J>
+__device__ __forceinline__ void join_warps(float2 (&mine)[W], float2* red, int s, int S, int lane, J join) {
+#pragma unroll
+  for (int j = 0; j < W; ++j) red[(s * W + j) * 32 + lane] = mine[j];
+  __syncthreads();
+  float2* res = red + S * W * 32;
+  for (int j = s; j < W; j += S) res[j * 32 + lane] = join(red + j * 32 + lane, W * 32);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < W; ++j) mine[j] = res[j * 32 + lane];
+}
+// component j of pairs of tokens (W = 1: a sum over the pair of channels is one number)
+template <int W>
+__device__ __forceinline__ float token(const float2* p, int j) {
+  return W == 1 ? p[0].x : (j & 1) ? p[j / 2].y : p[j / 2].x;
+}
+template <int W>
+__device__ __forceinline__ void set_token(float2* p, int j, float v) {
+  if (W == 1) p[0] = f2(v);
+  else if (j & 1) p[j / 2].y = v;
+  else p[j / 2].x = v;
+}
+// after sums over slots: W = 1 adds its two channels
+template <int W>
+__device__ __forceinline__ void fold_slot(float2* p) {
+  if (W == 1) p[0] = f2(p[0].x + p[0].y);
+}
 
 template <typename T, int W, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) ln_chan_fwd_kernel(LnArgs a) {
-  extern __shared__ __align__(16) float2 ln_sm[];  // [C] (w, b), then two buffers [P][S][W][32] (sum, M2)
-  const int lane = threadIdx.x, s = threadIdx.y, S = blockDim.y, P = blockDim.z;
-  for (int c = threadIdx.x + 32 * (threadIdx.y + S * threadIdx.z); c < a.C; c += 32 * S * P)
-    ln_sm[c] = make_float2(load_param(a.w, a.pdt, c, 1.f), load_param(a.b, a.pdt, c, 0.f));
-  float2* red = ln_sm + a.C + threadIdx.z * S * W * 32;
-  const int buffer = P * S * W * 32;
-  int turn = 0;
+  using Word = TokenWord<T, W>;
+  using P = typename Word::P;
+  constexpr int CPT = chan_cpt<T, W>(), kPairs = Word::kPairs, kChans = Word::kChans, kSlots = CPT / kChans;
+  extern __shared__ __align__(16) float ln_sm[];  // [C] (w, w, b, b), then [P] x join_warps' pairs
+  const int lane = threadIdx.x, s = threadIdx.y, S = blockDim.y, tiles_cta = blockDim.z;
+  float4* par = reinterpret_cast<float4*>(ln_sm);
+  for (int c = threadIdx.x + 32 * (threadIdx.y + S * threadIdx.z); c < a.C; c += 32 * S * tiles_cta) {
+    const float w = load_param(a.w, a.pdt, c, 1.f), b = load_param(a.b, a.pdt, c, 0.f);
+    par[c] = make_float4(w, w, b, b);
+  }
+  float2* red = reinterpret_cast<float2*>(par + a.C) + threadIdx.z * (S + 1) * W * 32;
   __syncthreads();
   const long long per = (a.inner + 32 * W - 1) / (32 * W), tiles = a.outer * per;
   const float rc = 1.f / (float)a.C;
-  const int mine = s < a.C ? (a.C - s + S - 1) / S : 0;  // channels of this warp
-  for (long long base = (long long)blockIdx.x * P; base < tiles; base += (long long)gridDim.x * P) {
+  const int share = a.C / S, more = a.C - share * S;  // warp i has share channels, one more where i < more
+  const int mine = share + (s < more ? 1 : 0);
+  const float rmine = 1.f / (float)mine;
+  for (long long base = (long long)blockIdx.x * tiles_cta; base < tiles; base += (long long)gridDim.x * tiles_cta) {
     const long long tile = base + threadIdx.z;
     const long long o = tile / per, v = (tile - o * per) * (32 * W) + lane * W;
-    const bool in = tile < tiles && v < a.inner;  // inner is even where W = 2
+    const bool in = tile < tiles && v < a.inner;  // inner is a multiple of W
     const long long at = (o * a.C + s) * a.inner + v, step = (long long)S * a.inner;
-    Word<T, W> x[kChanCpt];
+    Word x[kSlots];
     const T* px = static_cast<const T*>(a.x) + at;
 #pragma unroll
-    for (int k = 0; k < kChanCpt; ++k, advance(px, step)) x[k].load(px, in && k < mine);
-    float mean[W], m2[W];
+    for (int k = 0; k < kSlots; ++k, advance(px, step * kChans)) x[k].load(px, in ? mine - k * kChans : 0, step);
+    // this warp's mean and squares about it; the warps' join below (Chan, Golub and LeVeque)
+    float2 nm[kPairs], m2[kPairs];
 #pragma unroll
-    for (int j = 0; j < W; ++j) mean[j] = m2[j] = 0.f;
+    for (int j = 0; j < kPairs; ++j) nm[j] = m2[j] = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < kChanCpt; ++k) {
-      float f[W];
-      x[k].get(f);
+    for (int k = 0; k < kSlots; ++k)
 #pragma unroll
-      for (int j = 0; j < W; ++j) mean[j] += f[j];
-    }
-    if (S == 1) {
+      for (int j = 0; j < kPairs; ++j) nm[j] = P::plus(x[k].w[j], nm[j]);
+    fold_slot<W>(nm);
 #pragma unroll
-      for (int j = 0; j < W; ++j) mean[j] *= rc;
-    } else {
-      // the warp's own mean for its own squares; both join below (Chan, Golub and LeVeque)
-      const float rm = mine > 0 ? 1.f / (float)mine : 0.f;
+    for (int j = 0; j < kPairs; ++j) nm[j] = __fmul2_rn(nm[j], f2(-rmine));
 #pragma unroll
-      for (int j = 0; j < W; ++j) mean[j] *= rm;
-    }
+    for (int k = 0; k < kSlots; ++k)
+      if (k * kChans < mine) {
+        x[k].again();
 #pragma unroll
-    for (int k = 0; k < kChanCpt; ++k)
-      if (k < mine) {
-        float f[W];
-        renew(x[k].v);
-        x[k].get(f);
-#pragma unroll
-        for (int j = 0; j < W; ++j) m2[j] = fmaf(f[j] - mean[j], f[j] - mean[j], m2[j]);
-      }
-    if (S > 1) {
-      float2* r = red + turn * buffer;
-      turn ^= 1;
-#pragma unroll
-      for (int j = 0; j < W; ++j) r[(s * W + j) * 32 + lane] = make_float2(mean[j], m2[j]);
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < W; ++j) {
-        float sum = 0.f, sq = 0.f;
-        for (int i = 0; i < S; ++i) sum = fmaf((float)((a.C - i + S - 1) / S), r[(i * W + j) * 32 + lane].x, sum);
-        mean[j] = sum * rc;
-        for (int i = 0; i < S; ++i) {
-          const float2 p = r[(i * W + j) * 32 + lane];
-          const float d = p.x - mean[j];
-          sq += fmaf((float)((a.C - i + S - 1) / S) * d, d, p.y);
+        for (int j = 0; j < kPairs; ++j) {
+          float2 d = P::plus(x[k].w[j], nm[j]);
+          if (W == 1 && k * kChans + 1 >= mine) d.y = 0.f;
+          m2[j] = __ffma2_rn(d, d, m2[j]);
         }
-        m2[j] = sq;
       }
-    }
-    float rstd[W];
+    fold_slot<W>(m2);
+    float2 rstd[kPairs];
+    float2 st[W];
 #pragma unroll
-    for (int j = 0; j < W; ++j) rstd[j] = rsqrtf(m2[j] * rc + a.eps);
+    for (int j = 0; j < W; ++j) st[j] = make_float2(token<W>(nm, j), token<W>(m2, j));
+    if (S > 1) {
+      join_warps<W>(st, red, s, S, lane, [=](const float2* p, int stride) {
+        float sum = 0.f, sq = 0.f;
+        for (int i = 0; i < S; ++i) sum = fmaf((float)(share + (i < more ? 1 : 0)), p[i * stride].x, sum);
+        const float m = sum * rc;  // of -x, as nm
+        for (int i = 0; i < S; ++i) {
+          const float d = p[i * stride].x - m;
+          sq += fmaf((float)(share + (i < more ? 1 : 0)) * d, d, p[i * stride].y);
+        }
+        return make_float2(m, sq);
+      });
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      st[j].y = rsqrtf(st[j].y * rc + a.eps);
+      set_token<W>(nm, j, st[j].x);
+      set_token<W>(rstd, j, st[j].y);
+    }
     if (in) {
       T* y = static_cast<T*>(a.y) + at;
 #pragma unroll
-      for (int k = 0; k < kChanCpt; ++k, advance(y, step))
-        if (k < mine) {
-          const float2 wb = lds2(ln_sm + k * S + s);
-          float f[W];
-          renew(x[k].v);
-          x[k].get(f);
+      for (int k = 0; k < kSlots; ++k, advance(y, step * kChans))
+        if (k * kChans < mine) {
+          float4 wb = lds4(par + k * kChans * S + s);
+          if (W == 1 && k * kChans + 1 < mine) {
+            const float4 next = lds4(par + (k * kChans + 1) * S + s);
+            wb.y = next.y;
+            wb.w = next.w;
+          }
+          float2 f[kPairs];
+          x[k].again();
 #pragma unroll
-          for (int j = 0; j < W; ++j) f[j] = fmaf((f[j] - mean[j]) * rstd[j], wb.x, wb.y);
-          Word<T, W>::store(y, f);
+          for (int j = 0; j < kPairs; ++j)
+            f[j] = __ffma2_rn(__fmul2_rn(P::plus(x[k].w[j], nm[j]), rstd[j]), make_float2(wb.x, wb.y),
+                              make_float2(wb.z, wb.w));
+          Word::store(y, mine - k * kChans, step, f);
         }
       if (a.stats != nullptr && s == 0) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) a.stats[o * a.inner + v + j] = make_float2(mean[j], rstd[j]);
+        for (int j = 0; j < W; ++j) a.stats[o * a.inner + v + j] = make_float2(-st[j].x, st[j].y);
       }
     }
   }
 }
 
-// Sums over the 32 lanes of 32 values each: lane l returns the sum of value l.  Halves
-// change places at distances 16, 8, ..., 1: 31 shuffles instead of 160.
-__device__ __forceinline__ float transpose_sum(float (&v)[32], int lane) {
+// Sums over the 32 lanes of N values each: lane l returns the sum of value l % N.  Halves
+// change places at distances N / 2 .. 1: N - 1 shuffles (and one for N = 16) instead of 5 N.
+template <int N>
+__device__ __forceinline__ float transpose_sum(float (&v)[N], int lane) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = N / 2; o > 0; o >>= 1) {
     const bool up = lane & o;
 #pragma unroll
     for (int i = 0; i < o; ++i) {
@@ -699,111 +874,130 @@ __device__ __forceinline__ float transpose_sum(float (&v)[32], int lane) {
       v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
     }
   }
+  if (N == 16) v[0] += __shfl_xor_sync(0xffffffffu, v[0], 16);
   return v[0];
 }
 
 template <typename T, int W, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) ln_chan_bwd_kernel(LnArgs a) {
-  extern __shared__ __align__(16) float2 ln_sm[];  // [C] (w, -), then two buffers [P][S][W][32] of sums
-  const int lane = threadIdx.x, s = threadIdx.y, S = blockDim.y, P = blockDim.z;
-  float* wsm = reinterpret_cast<float*>(ln_sm);
-  for (int c = threadIdx.x + 32 * (threadIdx.y + S * threadIdx.z); c < a.C; c += 32 * S * P)
-    wsm[c] = load_param(a.w, a.pdt, c, 1.f);
-  float2* red = ln_sm + a.C + threadIdx.z * S * W * 32;
-  const int buffer = P * S * W * 32;
-  int turn = 0;
+  using Word = TokenWord<T, W>;
+  using P = typename Word::P;
+  constexpr int CPT = chan_cpt<T, W>(), kPairs = Word::kPairs, kChans = Word::kChans, kSlots = CPT / kChans;
+  extern __shared__ __align__(16) float ln_sm[];  // [C] (w, w), then [P] x join_warps' pairs
+  const int lane = threadIdx.x, s = threadIdx.y, S = blockDim.y, tiles_cta = blockDim.z;
+  float2* par = reinterpret_cast<float2*>(ln_sm);
+  for (int c = threadIdx.x + 32 * (threadIdx.y + S * threadIdx.z); c < a.C; c += 32 * S * tiles_cta)
+    par[c] = f2(load_param(a.w, a.pdt, c, 1.f));
+  float2* red = par + a.C + threadIdx.z * (S + 1) * W * 32;
   __syncthreads();
   const long long per = (a.inner + 32 * W - 1) / (32 * W), tiles = a.outer * per;
   const float rc = 1.f / (float)a.C;
-  const int mine = s < a.C ? (a.C - s + S - 1) / S : 0;
-  float dw = 0.f, db = 0.f;  // of channel lane * S + s
-  for (long long base = (long long)blockIdx.x * P; base < tiles; base += (long long)gridDim.x * P) {
+  const int mine = a.C / S + (s < a.C % S ? 1 : 0);
+  const auto weight = [=](int k) {  // of slot k
+    float2 w = lds2(par + k * kChans * S + s);
+    if (W == 1 && k * kChans + 1 < mine) w.y = lds2(par + (k * kChans + 1) * S + s).y;
+    return w;
+  };
+  float dw = 0.f, db = 0.f;  // of channel (lane % CPT) * S + s
+  for (long long base = (long long)blockIdx.x * tiles_cta; base < tiles; base += (long long)gridDim.x * tiles_cta) {
     const long long tile = base + threadIdx.z;
     const long long o = tile / per, v = (tile - o * per) * (32 * W) + lane * W;
     const bool in = tile < tiles && v < a.inner;
     const long long at = (o * a.C + s) * a.inner + v, step = (long long)S * a.inner;
-    Word<T, W> x[kChanCpt], d[kChanCpt];
+    Word x[kSlots], d[kSlots];
     const T *px = static_cast<const T*>(a.x) + at, *pd = static_cast<const T*>(a.dy) + at;
 #pragma unroll
-    for (int k = 0; k < kChanCpt; ++k, advance(px, step), advance(pd, step)) {
-      x[k].load(px, in && k < mine);
-      d[k].load(pd, in && k < mine);
+    for (int k = 0; k < kSlots; ++k, advance(px, step * kChans), advance(pd, step * kChans)) {
+      x[k].load(px, in ? mine - k * kChans : 0, step);
+      d[k].load(pd, in ? mine - k * kChans : 0, step);
     }
-    float2 st[W], sum[W];
+    float2 nm[kPairs], r[kPairs], s1[kPairs], s2[kPairs];
 #pragma unroll
     for (int j = 0; j < W; ++j) {
-      st[j] = in ? a.stats[o * a.inner + v + j] : make_float2(0.f, 0.f);
-      sum[j] = make_float2(0.f, 0.f);
+      const float2 st = in ? a.stats[o * a.inner + v + j] : make_float2(0.f, 0.f);
+      set_token<W>(nm, j, -st.x);
+      set_token<W>(r, j, st.y);
     }
 #pragma unroll
-    for (int k = 0; k < kChanCpt; ++k)
-      if (k < mine) {
-        const float w = lds1(wsm + k * S + s);
-        float f[W], g[W];
-        x[k].get(f);
-        d[k].get(g);
+    for (int j = 0; j < kPairs; ++j) s1[j] = s2[j] = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-          const float gw = g[j] * w;
-          sum[j].x += gw;
-          sum[j].y = fmaf(gw, (f[j] - st[j].x) * st[j].y, sum[j].y);
+    for (int k = 0; k < kSlots; ++k)
+      if (k * kChans < mine) {
+        const float2 w = weight(k);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          // sum of g (x - mean): the common r is multiplied once, below.  An absent second
+          // channel (W = 1) has dy = 0.
+          const float2 gw = __fmul2_rn(P::value(d[k].w[j]), w);
+          s1[j] = __fadd2_rn(s1[j], gw);
+          s2[j] = __ffma2_rn(gw, P::plus(x[k].w[j], nm[j]), s2[j]);
         }
       }
+    fold_slot<W>(s1);
+    fold_slot<W>(s2);
     if (S > 1) {
-      float2* r = red + turn * buffer;
-      turn ^= 1;
+      float2 sums[W];
 #pragma unroll
-      for (int j = 0; j < W; ++j) r[(s * W + j) * 32 + lane] = sum[j];
-      __syncthreads();
+      for (int j = 0; j < W; ++j) sums[j] = make_float2(token<W>(s1, j), token<W>(s2, j));
+      join_warps<W>(sums, red, s, S, lane, [=](const float2* p, int stride) {
+        float2 t = p[0];
+        for (int i = 1; i < S; ++i) t = __fadd2_rn(t, p[i * stride]);
+        return t;
+      });
 #pragma unroll
       for (int j = 0; j < W; ++j) {
-        sum[j] = make_float2(0.f, 0.f);
-        for (int i = 0; i < S; ++i) {
-          const float2 p = r[(i * W + j) * 32 + lane];
-          sum[j].x += p.x;
-          sum[j].y += p.y;
-        }
+        set_token<W>(s1, j, sums[j].x);
+        set_token<W>(s2, j, sums[j].y);
       }
     }
-    float pw[kChanCpt], pb[kChanCpt];
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+      s1[j] = __fmul2_rn(s1[j], f2(-rc));                    // -mean(g)
+      s2[j] = __fmul2_rn(__fmul2_rn(s2[j], r[j]), f2(-rc));  // -mean(g xh)
+    }
+    float pw[CPT], pb[CPT];
     T* dx = static_cast<T*>(a.y) + at;
 #pragma unroll
-    for (int k = 0; k < kChanCpt; ++k, advance(dx, step)) {
-      pw[k] = pb[k] = 0.f;
-      if (k < mine) {
-        const float w = lds1(wsm + k * S + s);
-        float f[W], g[W];
-        renew(x[k].v);
-        renew(d[k].v);
-        x[k].get(f);
-        d[k].get(g);
+    for (int k = 0; k < kSlots; ++k, advance(dx, step * kChans)) {
+      float2 tw = make_float2(0.f, 0.f), tb = tw;
+      if (k * kChans < mine) {
+        const float2 w = weight(k);
+        float2 f[kPairs];
+        x[k].again();
+        d[k].again();
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-          const float xh = (f[j] - st[j].x) * st[j].y;
-          pw[k] = fmaf(g[j], xh, pw[k]);
-          pb[k] += g[j];
-          f[j] = st[j].y * (fmaf(g[j], w, -sum[j].x * rc) - xh * (sum[j].y * rc));
+        for (int j = 0; j < kPairs; ++j) {
+          const float2 g = P::value(d[k].w[j]), xh = __fmul2_rn(P::plus(x[k].w[j], nm[j]), r[j]);
+          tw = __ffma2_rn(g, xh, tw);
+          tb = __fadd2_rn(tb, g);
+          f[j] = __fmul2_rn(__ffma2_rn(xh, s2[j], __ffma2_rn(g, w, s1[j])), r[j]);
         }
-        if (in) Word<T, W>::store(dx, f);
+        if (in) Word::store(dx, mine - k * kChans, step, f);
+      }
+      if constexpr (W == 1) {
+        pw[2 * k] = tw.x;
+        pw[2 * k + 1] = tw.y;
+        pb[2 * k] = tb.x;
+        pb[2 * k + 1] = tb.y;
+      } else {
+        pw[k] = tw.x + tw.y;
+        pb[k] = tb.x + tb.y;
       }
     }
     if (a.part != nullptr) {
-      dw += transpose_sum(pw, lane);
-      db += transpose_sum(pb, lane);
+      dw += transpose_sum<CPT>(pw, lane);
+      db += transpose_sum<CPT>(pb, lane);
     }
   }
   if (a.part == nullptr) return;
-  // the CTA's P tiles, in order, then one partial per CTA
+  // the CTA's tiles, in order, then one partial per CTA
   __syncthreads();
-  float2* acc = ln_sm + a.C;  // [P][S][32]
+  float2* acc = par + a.C;  // [P][S][32]
   acc[(threadIdx.z * S + s) * 32 + lane] = make_float2(dw, db);
   __syncthreads();
   if (threadIdx.z == 0 && lane < mine) {
     float2 t = acc[s * 32 + lane];
-    for (int p = 1; p < P; ++p) {
-      t.x += acc[(p * S + s) * 32 + lane].x;
-      t.y += acc[(p * S + s) * 32 + lane].y;
-    }
+    for (int p = 1; p < tiles_cta; ++p) t = __fadd2_rn(t, acc[(p * S + s) * 32 + lane]);
     float* part = a.part + (long long)blockIdx.x * 2 * a.C;
     part[lane * S + s] = t.x;
     part[a.C + lane * S + s] = t.y;
@@ -815,151 +1009,152 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) ln_chan_bwd_k
 enum LnForm { kRows, kChan, kAny };
 struct LnPlan {
   LnForm form;
-  int vec;      // kRows: 16-byte vectors; kChan: two 16-bit tokens per word
-  int ept;      // kRows: elements per thread
-  int G;        // kRows: threads per row
-  int threads;  // kRows: of a CTA
-  int S, P;     // kChan: warps per tile, tiles per CTA
+  int vec;          // kRows: elements per word; kChan: tokens per word
+  int ept;          // kRows: elements per thread
+  int G;            // kRows: threads per row
+  int threads;      // kRows: of a CTA
+  int S, P;         // kChan: warps per tile, tiles per CTA
   long long units;  // CTA-sized pieces of work
 };
 
-// Rows: as few threads per row as hold it at 8 elements each (2 vectors of fp32, 1 of
-// 16-bit data), more elements only past the largest CTA.  Backward threads also hold
-// their columns' weight-grad sums, so their CTAs and elements are fewer.
-LnPlan plan_rows(long long tokens, int C, bool vec, bool bwd) {
+// Rows: a power of two of threads with 8 elements each up to 256 columns, one warp with 16,
+// 24 or 32 up to 1024, then as many warps with 32 as the CTA has: 8192 columns.
+LnPlan plan_rows(long long tokens, int C, int vec) {
   LnPlan p{};
-  const int most = bwd ? 512 : 1024;
-  p.vec = vec;
-  for (p.ept = 8; p.ept <= (bwd ? 16 : 32); p.ept *= 2) {
-    const int need = (C + p.ept - 1) / p.ept;
-    if (!vec && p.ept > 8) break;  // single elements take a register each
-    if (need > most) continue;
-    p.G = 1;
-    while (p.G < need && p.G < 32) p.G *= 2;
-    if (need > 32) p.G = (need + 31) / 32 * 32;
-    p.threads = p.G <= 32 ? 256 : std::max(1, 256 / p.G) * p.G;
-    p.form = kRows;
-    const int rows = p.threads / p.G;
-    p.units = (tokens + rows - 1) / rows;
-    return p;
-  }
   p.form = kAny;
+  // single elements take a register and a predicate each: 8 per thread, on more threads
+  if (C > kRowThreads * (vec == 1 ? 8 : 32)) return p;
+  p.form = kRows;
+  p.vec = vec;
+  p.ept = vec == 1 || C <= 256 ? 8 : C <= 512 ? 16 : C <= 768 ? 24 : 32;
+  const int need = (C + p.ept - 1) / p.ept;
+  p.G = 1;
+  while (p.G < need && p.G < 32) p.G *= 2;
+  if (need > 32) p.G = (need + 31) / 32 * 32;
+  p.threads = kRowThreads / p.G * p.G;
+  const int rows = p.threads / p.G;
+  p.units = (tokens + rows - 1) / rows;
   return p;
 }
 
-// Channels first: 32 channels per thread, up to 32 warps forward (1024 channels), 16
-// backward (512: its threads hold x and dy).
-LnPlan plan_chan(long long outer, long long inner, int C, bool pair, bool bwd) {
+// Channels first: the widest word that the alignment allows and whose tile has enough
+// warps for C: 32 forward, 16 backward (its threads hold x and dy).
+LnPlan plan_chan(long long outer, long long inner, int C, size_t esz, size_t align, bool bwd) {
   LnPlan p{};
-  p.S = (C + kChanCpt - 1) / kChanCpt;
-  if (p.S > (bwd ? 16 : 32)) {
-    p.form = kAny;
+  p.form = kAny;
+  const int most = bwd ? 16 : 32;
+  for (int w = (int)(8 / esz); w >= 1; w /= 2) {
+    if (inner % w != 0 || align % (w * esz) != 0) continue;
+    const int cpt = w * (int)esz == 8 ? 16 : 32;
+    p.S = (C + cpt - 1) / cpt;
+    if (p.S > most) continue;
+    p.form = kChan;
+    p.vec = w;
+    p.P = std::max(1, 4 / p.S);
+    p.units = (outer * ((inner + 32 * w - 1) / (32 * w)) + p.P - 1) / p.P;
     return p;
   }
-  p.form = kChan;
-  p.vec = pair;
-  p.P = std::max(1, 4 / p.S);
-  const long long w = pair ? 64 : 32;
-  p.units = (outer * ((inner + w - 1) / w) + p.P - 1) / p.P;
   return p;
-}
-
-bool aligned_to(const LnArgs& a, size_t n) {
-  return ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.dy)) %
-          n) == 0;
 }
 
 template <typename T>
 LnPlan plan_ln(const LnArgs& a, bool bwd) {
-  if (a.inner == 1) return plan_rows(a.tokens, a.C, a.C % (16 / sizeof(T)) == 0 && aligned_to(a, 16), bwd);
-  return plan_chan(a.outer, a.inner, a.C, sizeof(T) == 2 && a.inner % 2 == 0 && aligned_to(a, 4), bwd);
+  // the largest power of two that divides every address, up to 16
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) |
+                         reinterpret_cast<uintptr_t>(a.dy) | 16;
+  const size_t align = (size_t)(bits & (~bits + 1));
+  if (a.inner > 1) return plan_chan(a.outer, a.inner, a.C, sizeof(T), align, bwd);
+  constexpr int V = 16 / sizeof(T);
+  int vec = 1;
+  if (a.C % V == 0 && align == 16) vec = V;
+  else if (sizeof(T) == 2 && a.C % 2 == 0 && align >= 4) vec = 2;
+  return plan_rows(a.tokens, a.C, vec);
 }
 
 // Most weight-grad partials that a call makes: one per CTA of the backward kernel, four
 // CTAs per SM; at least four tokens each, so that the partials stay small beside the data.
 int dw_parts(long long tokens) { return (int)std::max(1LL, std::min((long long)kSms * 4, (tokens + 3) / 4)); }
 
-template <typename T, int VEC, int EPT, int R, int THREADS>
-int launch_rows_fwd_as(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
-  // as many CTAs as the registers of the launch bounds let reside: 768 or 1024 threads
-  const long long cap = kSms * (long long)((R > 1 ? 768 : 1024) / p.threads);
-  ln_rows_fwd_kernel<T, VEC, EPT, R, THREADS>
-      <<<(unsigned)std::min((p.units + R - 1) / R, cap), p.threads, 0, s>>>(a, p.G);
+// Launches KERNEL<T, VEC, EPT, R> for a plan's vec and ept.
+template <typename T, int VEC, int EPT, int R>
+int launch_rows(const LnArgs& a, const LnPlan& p, bool bwd, int parts, cudaStream_t s) {
+  const size_t param = RowParam<T, VEC, EPT>::smem_bytes(p.G);
+  if (!bwd) {
+    auto kern = ln_rows_fwd_kernel<T, VEC, EPT, R>;
+    const int st = ensure_smem(kern, 2 * param);
+    if (st != MEDNEXT_OK) return st;
+    const long long cap = kSms * 3LL;  // resident by the launch bounds
+    kern<<<(unsigned)std::min((p.units + R - 1) / R, cap), p.threads, 2 * param, s>>>(a, p.G);
+  } else {
+    constexpr int RB = R > 2 ? 2 : 1;
+    auto kern = ln_rows_bwd_kernel<T, VEC, EPT, RB>;
+    const int slots = p.G < 32 ? p.threads / 32 : p.threads / p.G;
+    const size_t smem = std::max(param, a.part != nullptr ? (size_t)slots * 2 * a.C * sizeof(float) : 0);
+    const int st = ensure_smem(kern, smem);
+    if (st != MEDNEXT_OK) return st;
+    kern<<<parts, p.threads, smem, s>>>(a, p.G);
+  }
   return record_launch();
 }
-template <typename T, int VEC, int EPT>
-int launch_rows_fwd(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
-  if constexpr (EPT == 8) {
-    // four rows in flight per thread once every SM has that much to do
-    if (p.threads <= 256 && p.units >= kSms * 32) return launch_rows_fwd_as<T, VEC, EPT, 4, 256>(a, p, s);
-    if (p.threads <= 256) return launch_rows_fwd_as<T, VEC, EPT, 1, 256>(a, p, s);
+template <typename T, int VEC>
+int launch_rows_vec(const LnArgs& a, const LnPlan& p, bool bwd, int parts, cudaStream_t s) {
+  // rows in flight per thread (half as many backward), once every SM has that much to do
+  const bool many = p.units >= kSms * 12;
+  if (VEC == 1 || p.ept == 8)
+    return many ? launch_rows<T, VEC, 8, 4>(a, p, bwd, parts, s) : launch_rows<T, VEC, 8, 1>(a, p, bwd, parts, s);
+  if constexpr (VEC > 1) {
+    if (p.ept == 16)
+      return many ? launch_rows<T, VEC, 16, 2>(a, p, bwd, parts, s) : launch_rows<T, VEC, 16, 1>(a, p, bwd, parts, s);
+    if (p.ept == 24) return launch_rows<T, VEC, 24, 1>(a, p, bwd, parts, s);
+    return launch_rows<T, VEC, 32, 1>(a, p, bwd, parts, s);
   }
-  return launch_rows_fwd_as<T, VEC, EPT, 1, 1024>(a, p, s);
+  return MEDNEXT_ERR_UNSUPPORTED;  // not reached
 }
-template <typename T, int VEC, int EPT, int R, int THREADS>
-int launch_rows_bwd_as(const LnArgs& a, const LnPlan& p, int parts, cudaStream_t s) {
-  auto kern = ln_rows_bwd_kernel<T, VEC, EPT, R, THREADS>;
-  const int slots = p.G < 32 ? p.threads / 32 : p.threads / p.G;
-  const size_t smem = a.part != nullptr ? (size_t)slots * 2 * a.C * sizeof(float) : 0;
-  const int st = ensure_smem(kern, smem);
-  if (st != MEDNEXT_OK) return st;
-  kern<<<parts, p.threads, smem, s>>>(a, p.G);
-  return record_launch();
-}
-template <typename T, int VEC, int EPT>
-int launch_rows_bwd(const LnArgs& a, const LnPlan& p, int parts, cudaStream_t s) {
-  if constexpr (EPT == 8) {
-    if (p.threads <= 256 && p.units >= 2 * parts) return launch_rows_bwd_as<T, VEC, EPT, 2, 256>(a, p, parts, s);
-    if (p.threads <= 256) return launch_rows_bwd_as<T, VEC, EPT, 1, 256>(a, p, parts, s);
-  }
-  return launch_rows_bwd_as<T, VEC, EPT, 1, 512>(a, p, parts, s);
+template <typename T>
+int launch_rows_any_vec(const LnArgs& a, const LnPlan& p, bool bwd, int parts, cudaStream_t s) {
+  if (p.vec == 1) return launch_rows_vec<T, 1>(a, p, bwd, parts, s);
+  if constexpr (sizeof(T) == 2)
+    if (p.vec == 2) return launch_rows_vec<T, 2>(a, p, bwd, parts, s);
+  return launch_rows_vec<T, 16 / sizeof(T)>(a, p, bwd, parts, s);
 }
 
-size_t chan_smem(const LnPlan& p, int C) {
-  return ((size_t)C + 2 * (size_t)p.P * p.S * (p.vec ? 2 : 1) * 32) * sizeof(float2);
-}
-template <typename T, int W, int THREADS>
-int launch_chan_fwd_as(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
-  auto kern = ln_chan_fwd_kernel<T, W, THREADS>;
-  const size_t smem = chan_smem(p, a.C);
-  const int st = ensure_smem(kern, smem);
-  if (st != MEDNEXT_OK) return st;
-  const long long cap = kSms * (long long)std::max(1, 24 / (p.S * p.P));  // resident: 24 warps
-  kern<<<(unsigned)std::min(p.units, cap), dim3(32, p.S, p.P), smem, s>>>(a);
+template <typename T, int W, int FWD_THREADS, int BWD_THREADS>
+int launch_chan(const LnArgs& a, const LnPlan& p, bool bwd, int parts, cudaStream_t s) {
+  const size_t red = (size_t)p.P * (p.S + 1) * W * 32 * sizeof(float2);
+  const dim3 block(32, p.S, p.P);
+  if (!bwd) {
+    auto kern = ln_chan_fwd_kernel<T, W, FWD_THREADS>;
+    const size_t smem = (size_t)a.C * sizeof(float4) + red;
+    const int st = ensure_smem(kern, smem);
+    if (st != MEDNEXT_OK) return st;
+    const long long cap = kSms * (long long)std::max(1, 24 / (p.S * p.P));  // resident: 24 warps
+    kern<<<(unsigned)std::min(p.units, cap), block, smem, s>>>(a);
+  } else {
+    auto kern = ln_chan_bwd_kernel<T, W, BWD_THREADS>;
+    const size_t smem = (size_t)a.C * sizeof(float2) + red;
+    const int st = ensure_smem(kern, smem);
+    if (st != MEDNEXT_OK) return st;
+    kern<<<parts, block, smem, s>>>(a);
+  }
   return record_launch();
 }
 template <typename T, int W>
-int launch_chan_fwd(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
-  return p.S <= 8 ? launch_chan_fwd_as<T, W, 256>(a, p, s) : launch_chan_fwd_as<T, W, 1024>(a, p, s);
+int launch_chan_word(const LnArgs& a, const LnPlan& p, bool bwd, int parts, cudaStream_t s) {
+  return p.S <= 8 ? launch_chan<T, W, 256, 256>(a, p, bwd, parts, s) : launch_chan<T, W, 1024, 512>(a, p, bwd, parts, s);
 }
-template <typename T, int W, int THREADS>
-int launch_chan_bwd_as(const LnArgs& a, const LnPlan& p, int parts, cudaStream_t s) {
-  auto kern = ln_chan_bwd_kernel<T, W, THREADS>;
-  const size_t smem = chan_smem(p, a.C);
-  const int st = ensure_smem(kern, smem);
-  if (st != MEDNEXT_OK) return st;
-  kern<<<parts, dim3(32, p.S, p.P), smem, s>>>(a);
-  return record_launch();
-}
-template <typename T, int W>
-int launch_chan_bwd(const LnArgs& a, const LnPlan& p, int parts, cudaStream_t s) {
-  return p.S <= 8 ? launch_chan_bwd_as<T, W, 256>(a, p, parts, s) : launch_chan_bwd_as<T, W, 512>(a, p, parts, s);
+template <typename T>
+int launch_chan_any_word(const LnArgs& a, const LnPlan& p, bool bwd, int parts, cudaStream_t s) {
+  if (p.vec == 1) return launch_chan_word<T, 1>(a, p, bwd, parts, s);
+  if constexpr (sizeof(T) == 2)
+    if (p.vec == 4) return launch_chan_word<T, 4>(a, p, bwd, parts, s);
+  return launch_chan_word<T, 2>(a, p, bwd, parts, s);
 }
 
 template <typename T>
 int ln_fwd(const LnArgs& a, cudaStream_t s) {
-  constexpr int V = 16 / sizeof(T);
   const LnPlan p = plan_ln<T>(a, false);
-  if (p.form == kRows) {
-    if (p.ept == 8) return p.vec ? launch_rows_fwd<T, V, 8>(a, p, s) : launch_rows_fwd<T, 1, 8>(a, p, s);
-    if (p.ept == 16) return launch_rows_fwd<T, V, 16>(a, p, s);
-    return launch_rows_fwd<T, V, 32>(a, p, s);
-  }
-  if (p.form == kChan) {
-    if constexpr (sizeof(T) == 2)
-      if (p.vec) return launch_chan_fwd<T, 2>(a, p, s);
-    return launch_chan_fwd<T, 1>(a, p, s);
-  }
+  if (p.form == kRows) return launch_rows_any_vec<T>(a, p, false, 0, s);
+  if (p.form == kChan) return launch_chan_any_word<T>(a, p, false, 0, s);
   if (a.inner == 1) {
     ln_rows_any_fwd_kernel<T><<<(unsigned)std::min<long long>(a.tokens, kSms * 32), 256, 0, s>>>(a);
   } else {
@@ -971,22 +1166,15 @@ int ln_fwd(const LnArgs& a, cudaStream_t s) {
 
 template <typename T>
 int ln_bwd(const LnArgs& a, void* dw, void* db, cudaStream_t s) {
-  constexpr int V = 16 / sizeof(T);
   const LnPlan p = plan_ln<T>(a, true);
   // one CTA per resident slot (the launch bounds leave 512 threads), one partial per CTA
-  const int warps = p.form == kRows ? p.threads / 32 : p.S * p.P;
-  const long long slots = (long long)kSms * std::max(1, 16 / std::max(1, warps));
+  const int warps = p.form == kRows ? p.threads / 32 : std::max(1, p.S * p.P);
+  const long long slots = (long long)kSms * std::max(1, 16 / warps);
   int st, parts = (int)std::min<long long>(std::min<long long>(dw_parts(a.tokens), slots), std::max(1LL, p.units));
   if (p.form == kRows) {
-    if (p.ept == 8)
-      st = p.vec ? launch_rows_bwd<T, V, 8>(a, p, parts, s) : launch_rows_bwd<T, 1, 8>(a, p, parts, s);
-    else
-      st = launch_rows_bwd<T, V, 16>(a, p, parts, s);
+    st = launch_rows_any_vec<T>(a, p, true, parts, s);
   } else if (p.form == kChan) {
-    if constexpr (sizeof(T) == 2)
-      st = p.vec ? launch_chan_bwd<T, 2>(a, p, parts, s) : launch_chan_bwd<T, 1>(a, p, parts, s);
-    else
-      st = launch_chan_bwd<T, 1>(a, p, parts, s);
+    st = launch_chan_any_word<T>(a, p, true, parts, s);
   } else {
     // enough CTAs for the GPU over the columns and the parts
     const long long cols = a.inner == 1 ? (a.C + 31) / 32 : a.C;
