@@ -21,6 +21,7 @@ namespace {
 
 constexpr float kTinyMax = 127.f * 1.17549435e-38f;
 constexpr int kI8MaxK = 131072;
+constexpr int kI8Sms = 148;
 
 // The largest magnitude of a token as ordered bits: the bits of |x| as an unsigned
 // number order as |x| does, infinity above every number and NaN above infinity.
@@ -44,28 +45,206 @@ __device__ __forceinline__ int8_t quantize(float v, TokenScale s) {
 }
 
 // ------------------------------ quantisation ------------------------------
-// Four values of one token to four bytes.
-__device__ __forceinline__ uint32_t quantize4(float a, float b, float c, float d, TokenScale s) {
-  return (uint32_t)(uint8_t)quantize(a, s) | (uint32_t)(uint8_t)quantize(b, s) << 8 |
-         (uint32_t)(uint8_t)quantize(c, s) << 16 | (uint32_t)(uint8_t)quantize(d, s) << 24;
+// rint(v * inverse) as the low byte of the sum with 1.5 * 2^23 (the sum's unit is 1, so its
+// rounding is the rint): two fp32 instructions in place of a conversion.  The product is
+// rounded before the sum, as the definition says.  Scalar intrinsics: the packed
+// fp32 x 2 product and sum were fused into one multiply-add, which rounds some of 10^4
+// values the other way.
+constexpr float kRint = 12582912.f;
+__device__ __forceinline__ float2 scaled2(float2 v, float inverse_x, float inverse_y) {
+  return make_float2(__fadd_rn(__fmul_rn(v.x, inverse_x), kRint), __fadd_rn(__fmul_rn(v.y, inverse_y), kRint));
+}
+// Four bytes of a token at once; a token without a scale (infinity or NaN in it) is masked
+// to zeros by the caller.
+__device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
+  const uint32_t ab = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040);
+  const uint32_t cd = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040);
+  return __byte_perm(ab, cd, 0x5410);
 }
 
-// Any layout and width: one token per warp at a time, inner apart its elements, which are
-// read twice.
+// Packed pairs: the running maximum of magnitudes and the values.
+template <typename T>
+struct Mag {  // 16-bit types: two per word, their bits ordered as the numbers are
+  using Word = uint32_t;
+  using Max = uint32_t;
+  static __device__ __forceinline__ Max join(Max m, Word w) { return __vmaxu2(m, w & 0x7fff7fffu); }
+  static __device__ __forceinline__ uint32_t lo(Max m) { return abs_bits(unpack2<T>(m).x); }
+  static __device__ __forceinline__ uint32_t hi(Max m) { return abs_bits(unpack2<T>(m).y); }
+  static __device__ __forceinline__ float2 value(Word w) { return unpack2<T>(w); }
+};
+template <>
+struct Mag<float> {
+  using Word = float2;
+  using Max = uint2;
+  static __device__ __forceinline__ Max join(Max m, Word w) {
+    return make_uint2(max(m.x, abs_bits(w.x)), max(m.y, abs_bits(w.y)));
+  }
+  static __device__ __forceinline__ uint32_t lo(Max m) { return m.x; }
+  static __device__ __forceinline__ uint32_t hi(Max m) { return m.y; }
+  static __device__ __forceinline__ float2 value(Word w) { return w; }
+};
+
+// Rows whose start and length are multiples of 16 bytes: G threads (a power of two up to 32)
+// hold a row's NV 16-byte vectors each; x is read once.
+template <typename T, int NV>
+__global__ void __launch_bounds__(256) i8_quantize_rows_kernel(const T* __restrict__ x, int8_t* __restrict__ q,
+                                                               float* __restrict__ scale, long long tokens, int K,
+                                                               int pitch, int G) {
+  using M = Mag<T>;
+  constexpr int E = 16 / sizeof(T), kPairs = E / 2;
+  const int groups = 256 / G, gi = threadIdx.x / G, gl = threadIdx.x - gi * G;
+  // uniform over the CTA: every lane takes part in the shuffles
+  for (long long t0 = (long long)blockIdx.x * groups; t0 < tokens; t0 += (long long)gridDim.x * groups) {
+    const long long t = t0 + gi;
+    typename M::Word w[NV][kPairs];
+    typename M::Max m{};
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * G + gl) * E;
+      const uint4 r = t < tokens && c < K ? *reinterpret_cast<const uint4*>(x + t * K + c) : make_uint4(0, 0, 0, 0);
+      memcpy(w[v], &r, 16);
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) m = M::join(m, w[v][i]);
+    uint32_t most = max(M::lo(m), M::hi(m));
+    for (int o = G >> 1; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (t >= tokens) continue;
+    const TokenScale s = token_scale(most);
+    const uint32_t keep = most >= 0x7f800000u ? 0u : 0xffffffffu;
+    if (gl == 0) scale[t] = s.scale;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * G + gl) * E;
+      if (c >= pitch) continue;  // columns K .. pitch get the zeros that were not loaded
+      uint32_t b[E / 4];
+#pragma unroll
+      for (int i = 0; i < E / 4; ++i) {
+        const float2 f = scaled2(M::value(w[v][2 * i]), s.inverse, s.inverse),
+                     g = scaled2(M::value(w[v][2 * i + 1]), s.inverse, s.inverse);
+        b[i] = low_bytes(f.x, f.y, g.x, g.y) & keep;
+      }
+      if constexpr (E == 8) *reinterpret_cast<uint2*>(q + t * pitch + c) = make_uint2(b[0], b[1]);
+      else *reinterpret_cast<uint32_t*>(q + t * pitch + c) = b[0];
+    }
+  }
+}
+
+// Channels first: a lane owns W neighbouring tokens (two 16-bit elements of a word, else one)
+// and 32 channels in a row of them; warp s of a tile's S takes the pieces s, s + S, .. of 32
+// channels.  Each piece's load is a coalesced segment of a channel's row, each token's 32
+// bytes are two 16-byte stores: the transpose to token rows costs no shared memory.  With one
+// piece per warp x is read once; else the pieces are read again (from L2) to be scaled.
+// blockDim = (32, S, P), P tiles side by side.
+template <typename T, int W>
+__global__ void __launch_bounds__(1024) i8_quantize_chan_kernel(const T* __restrict__ x, int8_t* __restrict__ q,
+                                                                float* __restrict__ scale, int outer, int inner,
+                                                                int K, int pitch) {
+  extern __shared__ uint32_t i8_max[];  // [2][P][S][W][32]
+  const int lane = threadIdx.x, s = threadIdx.y, S = blockDim.y, P = blockDim.z;
+  const int per = (inner + 32 * W - 1) / (32 * W), pieces = (pitch + 31) / 32;  // pitch >= K
+  const long long tiles = (long long)outer * per;
+  int turn = 0;
+  for (long long base = (long long)blockIdx.x * P; base < tiles; base += (long long)gridDim.x * P) {
+    const long long tile = base + threadIdx.z;
+    const int o = (int)(tile / per), v = (int)(tile - (long long)o * per) * (32 * W) + lane * W;
+    const bool in = tile < tiles && v < inner;  // inner is even where W = 2
+    const T* px = x + (long long)o * K * inner + v;
+    uint32_t w[32];
+    const auto load = [&](int piece) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const int c = piece * 32 + k;
+        const bool ok = in && c < K;
+        const T* p = px + (long long)c * inner;
+        if constexpr (W == 2) w[k] = ok ? *reinterpret_cast<const uint32_t*>(p) : 0u;
+        else if constexpr (sizeof(T) == 4) w[k] = ok ? __float_as_uint(*p) : 0u;
+        else w[k] = ok ? (uint32_t)*reinterpret_cast<const uint16_t*>(p) : 0u;
+      }
+    };
+    uint32_t m = 0;  // magnitudes: W = 2 two 16-bit ones, else one
+    for (int piece = s; piece < pieces; piece += S) {
+      load(piece);
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        if constexpr (W == 2) m = __vmaxu2(m, w[k] & 0x7fff7fffu);
+        else m = max(m, w[k] & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fffu));
+      }
+    }
+    uint32_t most[W];
+    if constexpr (W == 2) {
+      most[0] = Mag<T>::lo(m);
+      most[W - 1] = Mag<T>::hi(m);
+    } else if constexpr (sizeof(T) == 4) {
+      most[0] = m;
+    } else {
+      most[0] = abs_bits(unpack2<T>(m).x);
+    }
+    if (S > 1) {
+      uint32_t* r = i8_max + (turn * P + threadIdx.z) * S * W * 32;
+      turn ^= 1;
+#pragma unroll
+      for (int j = 0; j < W; ++j) r[(s * W + j) * 32 + lane] = most[j];
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        for (int i = 0; i < S; ++i) most[j] = max(most[j], r[(i * W + j) * 32 + lane]);
+    }
+    TokenScale ts[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) ts[j] = token_scale(most[j]);
+    if (!in) continue;  // no barrier until the next tile's
+    const long long t = (long long)o * inner + v;
+    if (s == 0) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) scale[t + j] = ts[j].scale;
+    }
+    for (int piece = s; piece < pieces; piece += S) {
+      if (pieces > S) load(piece);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = piece * 32 + h * 16;
+        if (c >= pitch) break;
+        uint32_t b[W][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float2 f[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t word = w[h * 16 + i * 4 + e];
+            if constexpr (W == 2) f[e] = unpack2<T>(word);
+            else if constexpr (sizeof(T) == 4) f[e] = make_float2(__uint_as_float(word), 0.f);
+            else f[e] = make_float2(unpack2<T>(word).x, 0.f);
+            f[e] = scaled2(f[e], ts[0].inverse, ts[W - 1].inverse);
+          }
+          b[0][i] = low_bytes(f[0].x, f[1].x, f[2].x, f[3].x);
+          if constexpr (W == 2) b[1][i] = low_bytes(f[0].y, f[1].y, f[2].y, f[3].y);
+        }
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          const uint32_t keep = most[j] >= 0x7f800000u ? 0u : 0xffffffffu;
+          *reinterpret_cast<uint4*>(q + (t + j) * pitch + c) =
+              make_uint4(b[j][0] & keep, b[j][1] & keep, b[j][2] & keep, b[j][3] & keep);
+        }
+      }
+    }
+  }
+}
+
+// Rows of any alignment and width: one token per warp at a time, read twice.
 template <typename T>
 __global__ void __launch_bounds__(256) i8_quantize_any_kernel(const T* __restrict__ x, int8_t* __restrict__ q,
-                                                              float* __restrict__ scale, long long tokens,
-                                                              long long inner, int K, long long pitch) {
+                                                              float* __restrict__ scale, long long tokens, int K,
+                                                              int pitch) {
   const int lane = threadIdx.x & 31;
   for (long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); t < tokens; t += (long long)gridDim.x * 8) {
-    const long long o = t / inner;
-    const T* p = x + o * K * inner + (t - o * inner);
+    const T* p = x + t * K;
     uint32_t m = 0;
-    for (int k = lane; k < K; k += 32) m = max(m, abs_bits(to_acc<T>(p[k * inner])));
+    for (int k = lane; k < K; k += 32) m = max(m, abs_bits(to_acc<T>(p[k])));
     m = __reduce_max_sync(0xffffffffu, m);
     const TokenScale s = token_scale(m);
-    for (int k = lane; k < pitch; k += 32)
-      q[t * pitch + k] = k < K ? quantize(to_acc<T>(p[k * inner]), s) : (int8_t)0;
+    for (int k = lane; k < pitch; k += 32) q[t * pitch + k] = k < K ? quantize(to_acc<T>(p[k]), s) : (int8_t)0;
     if (lane == 0) scale[t] = s.scale;
   }
 }
@@ -320,11 +499,41 @@ int launch_gemm(const int8_t* q, const float* qs, long long q_pitch, const int8_
 long long pitch16(int64_t k) { return (k + 15) / 16 * 16; }
 
 template <typename T>
-int launch_quantize(const void* x, int8_t* q, float* scale, long long outer, int K, long long inner, long long pitch,
+int launch_quantize(const void* xv, int8_t* q, float* scale, long long outer, int K, long long inner, long long pitch,
                     cudaStream_t s) {
   const long long tokens = outer * inner;
-  i8_quantize_any_kernel<T><<<(unsigned)std::min<long long>((tokens + 7) / 8, 148 * 16), 256, 0, s>>>(
-      static_cast<const T*>(x), q, scale, tokens, inner, K, pitch);
+  const T* x = static_cast<const T*>(xv);
+  if (inner > 1) {
+    // two tokens per word where the alignment allows and the halved tiles still fill the GPU
+    const bool pair = sizeof(T) == 2 && inner % 2 == 0 && (reinterpret_cast<uintptr_t>(xv) & 3) == 0 &&
+                      outer * ((inner + 63) / 64) >= kI8Sms;
+    const int W = pair ? 2 : 1, S = std::min(32, (K + 31) / 32), P = std::max(1, 4 / S);
+    const long long tiles = outer * ((inner + 32 * W - 1) / (32 * W));
+    const unsigned grid = (unsigned)std::min<long long>((tiles + P - 1) / P, kI8Sms * 64);
+    const size_t smem = 2 * (size_t)P * S * W * 32 * sizeof(uint32_t);
+    if constexpr (sizeof(T) == 2)
+      if (pair) {
+        i8_quantize_chan_kernel<T, 2><<<grid, dim3(32, S, P), smem, s>>>(x, q, scale, (int)outer, (int)inner, K, (int)pitch);
+        return record_launch();
+      }
+    i8_quantize_chan_kernel<T, 1><<<grid, dim3(32, S, P), smem, s>>>(x, q, scale, (int)outer, (int)inner, K, (int)pitch);
+    return record_launch();
+  }
+  constexpr int E = 16 / sizeof(T);
+  const int vecs = (int)((pitch + E - 1) / E);
+  // the registers of a warp hold 16 vectors per lane
+  if (K % E == 0 && (reinterpret_cast<uintptr_t>(xv) & 15) == 0 && pitch - K < 16 && vecs <= 512) {
+    int G = 1;
+    while (G < 32 && G < vecs) G *= 2;
+    const int rows = 256 / G;
+    const unsigned grid = (unsigned)std::min<long long>((tokens + rows - 1) / rows, kI8Sms * 64);
+    if (vecs <= 32) i8_quantize_rows_kernel<T, 1><<<grid, 256, 0, s>>>(x, q, scale, tokens, K, (int)pitch, G);
+    else if (vecs <= 128) i8_quantize_rows_kernel<T, 4><<<grid, 256, 0, s>>>(x, q, scale, tokens, K, (int)pitch, G);
+    else i8_quantize_rows_kernel<T, 16><<<grid, 256, 0, s>>>(x, q, scale, tokens, K, (int)pitch, G);
+    return record_launch();
+  }
+  i8_quantize_any_kernel<T><<<(unsigned)std::min<long long>((tokens + 7) / 8, kI8Sms * 16), 256, 0, s>>>(
+      x, q, scale, tokens, K, (int)pitch);
   return record_launch();
 }
 
