@@ -446,6 +446,213 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   if (warp == 1) tmem_dealloc(tmem, tmem_cols);
 }
 
+// ------------------------------ narrow products in one kernel ------------------------------
+// Channels first with weights that stay in shared memory: the product is bound by the
+// bytes of x and y, so x is read, quantised, multiplied and written by the same CTA, and
+// no 8-bit rows go through memory (the two-kernel form reads and writes K bytes per token
+// more, and its accumulators pass through TMEM: 248 us against this kernel's TIMES us for
+// 32 -> 64 channels at 128^3, where x and y take 62 us of bandwidth).
+//
+// A tile is 32 W tokens.  Warp s of S = ceil(K / 32) quantises channels 32 s .. of it as
+// i8_quantize_chan_kernel does, into token rows in shared memory.  Then the warps share the
+// output channels, 16 at a time: mma.sync m16n8k32 with the weights as A, so that sums stay
+// in the registers of the thread that stores them.  Column n of the four B fragments of 32
+// tokens is token 8 (n / 2) + 2 j + n % 2 of them: a thread's columns 2 t, 2 t + 1 of
+// fragments j = 0 .. 3 are 8 neighbouring tokens, one 16-byte store of 16-bit data.
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+struct I8NarrowArgs {
+  const void* x;
+  const int8_t* w;
+  const float* ws;
+  const float* bias;  // or NULL
+  void* y;
+  long long w_pitch;
+  int outer, inner, K, N;
+  int vec;  // y's rows start on 16 bytes: 8 tokens per store
+};
+
+// Shared memory: weights [N16][row], per output channel (scale, bias), then per tile of the
+// CTA: token rows [32 W][row], their scales, and the warps' maxima [S][W][32].  row = K
+// rounded up to 32, plus 16: an odd number of 16-byte units, so that eight rows' ldmatrix
+// reads fall on different banks.
+__host__ __device__ __forceinline__ int narrow_row(int K) { return (K + 31) / 32 * 32 + 16; }
+__host__ __device__ __forceinline__ int narrow_tile_bytes(int K, int W) {
+  return 32 * W * narrow_row(K) + 32 * W * 4 + (K + 31) / 32 * W * 128;
+}
+__host__ __device__ __forceinline__ int narrow_weight_bytes(int K, int N) {
+  return (N + 15) / 16 * 16 * (narrow_row(K) + 8);
+}
+
+template <typename T, int W>
+__global__ void __launch_bounds__(512) i8_narrow_kernel(I8NarrowArgs a) {
+  extern __shared__ __align__(16) uint8_t i8_sm[];
+  const int lane = threadIdx.x, s = threadIdx.y, S = blockDim.y, P = blockDim.z;
+  const int row = narrow_row(a.K), n16 = (a.N + 15) / 16;
+  uint8_t* wsm = i8_sm;
+  float2* chan = reinterpret_cast<float2*>(i8_sm + n16 * 16 * row);
+  uint8_t* tile_sm = i8_sm + narrow_weight_bytes(a.K, a.N) + threadIdx.z * narrow_tile_bytes(a.K, W);
+  float* tscale = reinterpret_cast<float*>(tile_sm + 32 * W * row);
+  uint32_t* maxima = reinterpret_cast<uint32_t*>(tscale + 32 * W);
+  {
+    const int me = threadIdx.x + 32 * (threadIdx.y + S * threadIdx.z), all = 32 * S * P;
+    const int pieces = (row - 16) / 16;
+    for (int i = me; i < n16 * 16 * pieces; i += all) {
+      const int n = i / pieces, k = (i - n * pieces) * 16;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      // the last 16 bytes of a row may hold bytes past K: they meet zeros of x
+      if (n < a.N && k < a.K) v = *reinterpret_cast<const uint4*>(a.w + n * a.w_pitch + k);
+      *reinterpret_cast<uint4*>(wsm + n * row + k) = v;
+    }
+    for (int n = me; n < n16 * 16; n += all)
+      chan[n] = n < a.N ? make_float2(a.ws[n], a.bias != nullptr ? a.bias[n] : 0.f) : make_float2(0.f, 0.f);
+  }
+  __syncthreads();
+  const auto meet = [&] {
+    if (S > 1) __syncthreads();
+    else __syncwarp();
+  };
+  const int per = (a.inner + 32 * W - 1) / (32 * W);
+  const long long tiles = (long long)a.outer * per;
+  const uint32_t w_addr = smem_u32(wsm), t_addr = smem_u32(tile_sm);
+  const int g = lane >> 2, t4 = lane & 3;
+  // ldmatrix row addresses: A takes rows 0-7, 8-15 of the first 16 bytes, then of the second;
+  // B takes fragment j's two halves, then fragment j + 1's, rows being the permuted tokens
+  const uint32_t a_off = (uint32_t)((lane & 15) * row + (lane >> 4) * 16);
+  const int bn = lane & 7;
+  const uint32_t b_off = (uint32_t)((8 * (bn >> 1) + 2 * (lane >> 4) + (bn & 1)) * row + ((lane >> 3) & 1) * 16);
+  for (long long base = (long long)blockIdx.x * P; base < tiles; base += (long long)gridDim.x * P) {
+    const long long tile = base + threadIdx.z;
+    const int o = (int)(tile / per), v0 = (int)(tile - (long long)o * per) * (32 * W), v = v0 + lane * W;
+    const bool in = tile < tiles && v < a.inner;  // inner is even where W = 2
+    const T* px = static_cast<const T*>(a.x) + ((long long)o * a.K + s * 32) * a.inner + v;
+    const int mine = min(32, a.K - s * 32);
+    uint32_t x[32];
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      const bool ok = in && k < mine;
+      if constexpr (W == 2) x[k] = ok ? *reinterpret_cast<const uint32_t*>(px) : 0u;
+      else if constexpr (sizeof(T) == 4) x[k] = ok ? __float_as_uint(*px) : 0u;
+      else x[k] = ok ? (uint32_t)*reinterpret_cast<const uint16_t*>(px) : 0u;
+      px += a.inner;
+      asm volatile("" : "+l"(px));  // one address in flight, not 32
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      if constexpr (W == 2) m = __vmaxu2(m, x[k] & 0x7fff7fffu);
+      else m = max(m, x[k] & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fffu));
+    }
+    uint32_t most[W];
+    if constexpr (W == 2) {
+      most[0] = Mag<T>::lo(m);
+      most[W - 1] = Mag<T>::hi(m);
+    } else if constexpr (sizeof(T) == 4) {
+      most[0] = m;
+    } else {
+      most[0] = abs_bits(unpack2<T>(m).x);
+    }
+    if (S > 1) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) maxima[(s * W + j) * 32 + lane] = most[j];
+    }
+    meet();  // the maxima are there, and the last tile's rows are read
+    if (S > 1) {
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        for (int i = 0; i < S; ++i) most[j] = max(most[j], maxima[(i * W + j) * 32 + lane]);
+    }
+    TokenScale ts[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      ts[j] = token_scale(most[j]);
+      if (s == 0) tscale[lane * W + j] = ts[j].scale;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t b[W][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float2 f[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t word = x[h * 16 + i * 4 + e];
+          if constexpr (W == 2) f[e] = unpack2<T>(word);
+          else if constexpr (sizeof(T) == 4) f[e] = make_float2(__uint_as_float(word), 0.f);
+          else f[e] = make_float2(unpack2<T>(word).x, 0.f);
+          f[e] = scaled2(f[e], ts[0].inverse, ts[W - 1].inverse);
+        }
+        b[0][i] = low_bytes(f[0].x, f[1].x, f[2].x, f[3].x);
+        if constexpr (W == 2) b[1][i] = low_bytes(f[0].y, f[1].y, f[2].y, f[3].y);
+      }
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const uint32_t keep = most[j] >= 0x7f800000u ? 0u : 0xffffffffu;
+        *reinterpret_cast<uint4*>(tile_sm + (lane * W + j) * row + s * 32 + h * 16) =
+            make_uint4(b[j][0] & keep, b[j][1] & keep, b[j][2] & keep, b[j][3] & keep);
+      }
+    }
+    meet();
+    if (tile < tiles) {
+#pragma unroll 1
+      for (int part = 0; part < W; ++part) {  // 32 tokens at a time
+        const int tok = part * 32 + 8 * t4, vt = v0 + tok;
+        float sc[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sc[i] = tscale[tok + i];
+#pragma unroll 1
+        for (int mt = s; mt < n16; mt += S) {
+          int acc[4][4] = {};
+          for (int kb = 0; kb < row - 16; kb += 32) {
+            uint32_t fa[4], fb[2][4];
+            ldsm_x4(w_addr + (uint32_t)(mt * 16 * row + kb) + a_off, fa);
+            ldsm_x4(t_addr + (uint32_t)(part * 32 * row + kb) + b_off, fb[0]);
+            ldsm_x4(t_addr + (uint32_t)((part * 32 + 4) * row + kb) + b_off, fb[1]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma_s8(acc[j], fa, fb[j >> 1][(j & 1) * 2], fb[j >> 1][(j & 1) * 2 + 1]);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // channels g and g + 8
+            const int n = mt * 16 + h * 8 + g;
+            if (n >= a.N) continue;
+            const float2 c = chan[n];
+            float out[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) out[i] = fmaf((float)acc[i >> 1][h * 2 + (i & 1)] * sc[i], c.x, c.y);
+            T* y = static_cast<T*>(a.y) + ((long long)o * a.N + n) * a.inner + vt;
+            if (a.vec && vt + 8 <= a.inner) {
+              constexpr int E = 16 / sizeof(T);
+#pragma unroll
+              for (int i = 0; i < 8; i += E) *reinterpret_cast<uint4*>(y + i) = pack16<T>(out + i);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (vt + i < a.inner) y[i] = from_acc<T>(out[i]);
+            }
+          }
+        }
+      }
+    }
+  }
+}
+
+// Whether the one-kernel form covers K and N: its weights and one tile in 100 KB of shared
+// memory (two CTAs per SM), 16 warps.
+bool narrow_covers(int K, int N) {
+  return K <= 512 && narrow_weight_bytes(K, N) + narrow_tile_bytes(K, 2) <= 100 * 1024;
+}
+
 int num_sms() {
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
@@ -538,8 +745,39 @@ int launch_quantize(const void* xv, int8_t* q, float* scale, long long outer, in
 }
 
 template <typename T>
+int launch_narrow(const I8NarrowArgs& a, cudaStream_t s) {
+  const uintptr_t xb = reinterpret_cast<uintptr_t>(a.x);
+  const bool pair = sizeof(T) == 2 && a.inner % 2 == 0 && xb % 4 == 0;
+  const int W = pair ? 2 : 1, S = (a.K + 31) / 32;
+  int P = std::max(1, 4 / S);
+  while (P > 1 && narrow_weight_bytes(a.K, a.N) + P * narrow_tile_bytes(a.K, W) > 100 * 1024) --P;
+  const size_t smem = narrow_weight_bytes(a.K, a.N) + (size_t)P * narrow_tile_bytes(a.K, W);
+  const long long tiles = (long long)a.outer * ((a.inner + 32 * W - 1) / (32 * W));
+  // resident CTAs: 32 warps by registers, and what shared memory holds
+  const int per_sm = std::max(1, std::min(32 / (S * P), (int)(220 * 1024 / (smem + 1024))));
+  const unsigned grid = (unsigned)std::min<long long>((tiles + P - 1) / P, (long long)kI8Sms * per_sm);
+  auto run = [&](auto kern) {
+    const int st = ensure_smem(kern, smem);
+    if (st != MEDNEXT_OK) return st;
+    kern<<<grid, dim3(32, S, P), smem, s>>>(a);
+    return record_launch();
+  };
+  if constexpr (sizeof(T) == 2)
+    if (pair) return run(i8_narrow_kernel<T, 2>);
+  return run(i8_narrow_kernel<T, 1>);
+}
+
+template <typename T>
 int launch_linear(const void* x, const int8_t* w, const float* ws, long long w_pitch, const float* bias, void* y,
                   int8_t* q, float* qs, long long outer, int K, long long inner, int N, cudaStream_t s) {
+  if (inner > 1 && narrow_covers(K, N) && outer * ((inner + 63) / 64) >= kI8Sms) {
+    I8NarrowArgs a{};
+    a.x = x; a.w = w; a.ws = ws; a.bias = bias; a.y = y;
+    a.w_pitch = w_pitch;
+    a.outer = (int)outer; a.inner = (int)inner; a.K = K; a.N = N;
+    a.vec = inner % (16 / (long long)sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+    return launch_narrow<T>(a, s);
+  }
   int st = launch_quantize<T>(x, q, qs, outer, K, inner, pitch16(K), s);
   if (st != MEDNEXT_OK) return st;
   return launch_gemm<T>(q, qs, pitch16(K), w, ws, w_pitch, bias, y, outer * inner, inner, K, N, s);
