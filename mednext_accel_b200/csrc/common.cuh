@@ -391,6 +391,14 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool ab_bf16
          ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
+// Programmatic dependent launch: a kernel launched with launch_dependent() (plan.h) may start
+// while its predecessor in the stream still runs, once every CTA of that one has called
+// grid_dependents_go() or ended.  grid_dependency_wait() returns when the predecessor is
+// complete and its writes are visible: nothing of the predecessor's is read, and nothing
+// that it may read is written, before it.
+__device__ __forceinline__ void grid_dependents_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // 2^x and 1/x by the PTX approximate instructions (relative error about 2^-22;
 // denormal results flush to zero).
 __device__ __forceinline__ float ex2_approx(float x) {

@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(256) i8_quantize_rows_kernel(const T* __restri
                                                                int pitch, int G) {
   using M = Mag<T>;
   constexpr int E = 16 / sizeof(T), kPairs = E / 2;
+  grid_dependents_go();
   const int groups = 256 / G, gi = threadIdx.x / G, gl = threadIdx.x - gi * G;
   // uniform over the CTA: every lane takes part in the shuffles
   for (long long t0 = (long long)blockIdx.x * groups; t0 < tokens; t0 += (long long)gridDim.x * groups) {
@@ -131,31 +132,58 @@ __global__ void __launch_bounds__(256) i8_quantize_rows_kernel(const T* __restri
   }
 }
 
-// Channels first: a lane owns W neighbouring tokens (two 16-bit elements of a word, else one)
-// and 32 channels in a row of them; warp s of a tile's S takes the pieces s, s + S, .. of 32
-// channels.  Each piece's load is a coalesced segment of a channel's row, each token's 32
-// bytes are two 16-byte stores: the transpose to token rows costs no shared memory.  With one
-// piece per warp x is read once; else the pieces are read again (from L2) to be scaled.
-// blockDim = (32, S, P), P tiles side by side.
+// 16 channels of W tokens (packed pairs of tokens for W = 2) to 16 bytes per token.
 template <typename T, int W>
+__device__ __forceinline__ void quantize16(const uint32_t* w, const TokenScale (&ts)[W], uint32_t (&b)[W][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 f[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t word = w[i * 4 + e];
+      if constexpr (W == 2) f[e] = unpack2<T>(word);
+      else if constexpr (sizeof(T) == 4) f[e] = make_float2(__uint_as_float(word), 0.f);
+      else f[e] = make_float2(unpack2<T>(word).x, 0.f);
+      f[e] = scaled2(f[e], ts[0].inverse, ts[W - 1].inverse);
+    }
+    b[0][i] = low_bytes(f[0].x, f[1].x, f[2].x, f[3].x);
+    if constexpr (W == 2) b[1][i] = low_bytes(f[0].y, f[1].y, f[2].y, f[3].y);
+  }
+}
+
+// Channels first: a lane owns W neighbouring tokens (two 16-bit elements of a word, else one)
+// and CH channels in a row of them.  TX lanes lie along the tokens, 32 / TX along further
+// channels, so that a warp has a piece of 32 / TX * CH channels; warp s of a tile's S takes
+// the pieces s, s + S, ..  Each load is a segment of a channel's row, each token's bytes are
+// 16-byte stores: the transpose to token rows costs no shared memory.  With one piece per
+// warp x is read once; else the pieces are read again (from L2) to be scaled.
+// blockDim = (32, S, P), P tiles side by side.
+//
+// TX = 32, CH = 32 is for many tokens.  Few tokens (deep levels) leave most SMs without a tile
+// of that size: TX = 8, CH = 16 makes four times as many, in 16- or 32-byte segments
+// (2048 channels x 512 voxels bf16: 14.9 -> 6.3 us).
+template <typename T, int W, int TX, int CH>
 __global__ void __launch_bounds__(1024) i8_quantize_chan_kernel(const T* __restrict__ x, int8_t* __restrict__ q,
                                                                 float* __restrict__ scale, int outer, int inner,
                                                                 int K, int pitch) {
-  extern __shared__ uint32_t i8_max[];  // [2][P][S][W][32]
+  constexpr int kPiece = 32 / TX * CH;
+  extern __shared__ uint32_t i8_max[];  // [2][P][S][W][TX]
+  grid_dependents_go();
   const int lane = threadIdx.x, s = threadIdx.y, S = blockDim.y, P = blockDim.z;
-  const int per = (inner + 32 * W - 1) / (32 * W), pieces = (pitch + 31) / 32;  // pitch >= K
+  const int tx = lane % TX, cy = lane / TX;
+  const int per = (inner + TX * W - 1) / (TX * W), pieces = (pitch + kPiece - 1) / kPiece;  // pitch >= K
   const long long tiles = (long long)outer * per;
   int turn = 0;
   for (long long base = (long long)blockIdx.x * P; base < tiles; base += (long long)gridDim.x * P) {
     const long long tile = base + threadIdx.z;
-    const int o = (int)(tile / per), v = (int)(tile - (long long)o * per) * (32 * W) + lane * W;
+    const int o = (int)(tile / per), v = (int)(tile - (long long)o * per) * (TX * W) + tx * W;
     const bool in = tile < tiles && v < inner;  // inner is even where W = 2
     const T* px = x + (long long)o * K * inner + v;
-    uint32_t w[32];
+    uint32_t w[CH];
     const auto load = [&](int piece) {
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const int c = piece * 32 + k;
+      for (int k = 0; k < CH; ++k) {
+        const int c = piece * kPiece + cy * CH + k;
         const bool ok = in && c < K;
         const T* p = px + (long long)c * inner;
         if constexpr (W == 2) w[k] = ok ? *reinterpret_cast<const uint32_t*>(p) : 0u;
@@ -167,10 +195,15 @@ __global__ void __launch_bounds__(1024) i8_quantize_chan_kernel(const T* __restr
     for (int piece = s; piece < pieces; piece += S) {
       load(piece);
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
+      for (int k = 0; k < CH; ++k) {
         if constexpr (W == 2) m = __vmaxu2(m, w[k] & 0x7fff7fffu);
         else m = max(m, w[k] & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fffu));
       }
+    }
+#pragma unroll
+    for (int d = TX; d < 32; d *= 2) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, m, d);
+      m = W == 2 ? __vmaxu2(m, other) : max(m, other);
     }
     uint32_t most[W];
     if constexpr (W == 2) {
@@ -182,53 +215,44 @@ __global__ void __launch_bounds__(1024) i8_quantize_chan_kernel(const T* __restr
       most[0] = abs_bits(unpack2<T>(m).x);
     }
     if (S > 1) {
-      uint32_t* r = i8_max + (turn * P + threadIdx.z) * S * W * 32;
+      uint32_t* r = i8_max + (turn * P + threadIdx.z) * S * W * TX;
       turn ^= 1;
+      if (cy == 0) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) r[(s * W + j) * 32 + lane] = most[j];
+        for (int j = 0; j < W; ++j) r[(s * W + j) * TX + tx] = most[j];
+      }
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < W; ++j)
-        for (int i = 0; i < S; ++i) most[j] = max(most[j], r[(i * W + j) * 32 + lane]);
+        for (int i = 0; i < S; ++i) most[j] = max(most[j], r[(i * W + j) * TX + tx]);
     }
     TokenScale ts[W];
 #pragma unroll
     for (int j = 0; j < W; ++j) ts[j] = token_scale(most[j]);
-    if (!in) continue;  // no barrier until the next tile's
-    const long long t = (long long)o * inner + v;
-    if (s == 0) {
+    if (in) {
+      const long long t = (long long)o * inner + v;
+      if (s == 0 && cy == 0) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) scale[t + j] = ts[j].scale;
-    }
-    for (int piece = s; piece < pieces; piece += S) {
-      if (pieces > S) load(piece);
+        for (int j = 0; j < W; ++j) scale[t + j] = ts[j].scale;
+      }
+      for (int piece = s; piece < pieces; piece += S) {
+        if (pieces > S) load(piece);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int c = piece * 32 + h * 16;
-        if (c >= pitch) break;
-        uint32_t b[W][4];
+        for (int h = 0; h < CH / 16; ++h) {
+          const int c = piece * kPiece + cy * CH + h * 16;
+          if (c >= pitch) break;
+          uint32_t b[W][4];
+          quantize16<T, W>(w + h * 16, ts, b);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float2 f[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t word = w[h * 16 + i * 4 + e];
-            if constexpr (W == 2) f[e] = unpack2<T>(word);
-            else if constexpr (sizeof(T) == 4) f[e] = make_float2(__uint_as_float(word), 0.f);
-            else f[e] = make_float2(unpack2<T>(word).x, 0.f);
-            f[e] = scaled2(f[e], ts[0].inverse, ts[W - 1].inverse);
+          for (int j = 0; j < W; ++j) {
+            const uint32_t keep = most[j] >= 0x7f800000u ? 0u : 0xffffffffu;
+            *reinterpret_cast<uint4*>(q + (t + j) * pitch + c) =
+                make_uint4(b[j][0] & keep, b[j][1] & keep, b[j][2] & keep, b[j][3] & keep);
           }
-          b[0][i] = low_bytes(f[0].x, f[1].x, f[2].x, f[3].x);
-          if constexpr (W == 2) b[1][i] = low_bytes(f[0].y, f[1].y, f[2].y, f[3].y);
-        }
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-          const uint32_t keep = most[j] >= 0x7f800000u ? 0u : 0xffffffffu;
-          *reinterpret_cast<uint4*>(q + (t + j) * pitch + c) =
-              make_uint4(b[j][0] & keep, b[j][1] & keep, b[j][2] & keep, b[j][3] & keep);
         }
       }
     }
+    __syncwarp();  // whole again for the next tile's shuffles
   }
 }
 
@@ -237,6 +261,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) i8_quantize_any_kernel(const T* __restrict__ x, int8_t* __restrict__ q,
                                                               float* __restrict__ scale, long long tokens, int K,
                                                               int pitch) {
+  grid_dependents_go();
   const int lane = threadIdx.x & 31;
   for (long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); t < tokens; t += (long long)gridDim.x * 8) {
     const T* p = x + t * K;
@@ -258,31 +283,38 @@ __global__ void __launch_bounds__(256) i8_quantize_any_kernel(const T* __restric
 // voxel), rows take the weights as A (lane = output channel).
 //
 // Persistent, warp-specialised: warp 0 issues the TMA loads (a ring of 128-byte K
-// blocks), warp 1 owns TMEM and issues the MMAs into two accumulators in turn, warps 2-9
-// scale and store.  The waits and the exit follow the pointwise kernels' discipline: every wait
+// blocks), warp 1 owns TMEM and issues the MMAs into two to four accumulators in turn, two
+// groups of four warps scale and store: a tile each in turn where TMEM holds four, so that one
+// tile's latencies pass under the other's, else half of every tile each.  The waits and the exit follow the pointwise kernels' discipline: every wait
 // is bounded, and what is in flight is waited for before TMEM is freed.
 constexpr int kI8BM = 128, kI8BK = 128;
 constexpr int kI8Threads = 320, kI8EpiWarps = 8;
-constexpr int kI8MaxStages = 8;
+constexpr int kI8MaxStages = 8, kI8MaxAcc = 4;
 
 struct I8GemmArgs {
   const float* a_scale;  // of A's rows
   const float* b_scale;  // of B's rows
   const float* bias;     // of the output channels, or NULL
   void* y;
-  int a_rows, b_rows, K;
-  int inner;  // of y
-  int N;      // output channels
-  int bn, stages, a_tiles, b_tiles;
+  int a_rows, b_rows, K;  // a_rows of one sample
+  int N;                  // output channels
+  int bn, stages, accs;
+  int share;  // the two groups share each tile
+  int a_tiles, samples, b_tiles;  // a_tiles of one sample
 };
+
+// Staged stores (16-bit y whose rows are whole 16-byte units): an epilogue warp turns its 32
+// lanes x 32 columns into rows of 64 bytes in shared memory (64-byte swizzle) and sends them
+// by TMA.  Two buffers per warp.
+constexpr int kI8StageBytes = 32 * 64;
 
 struct I8Shared {
   uint64_t full[kI8MaxStages], empty[kI8MaxStages];
-  uint64_t tfull[2], tempty[2];
+  uint64_t tfull[kI8MaxAcc], tempty[kI8MaxAcc];
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
-  float2 col[kI8EpiWarps][32];  // (scale, bias) of an epilogue warp's 32 columns
+  float4 col[kI8EpiWarps][16];  // (scale, bias) of an epilogue warp's 32 columns
 };
 
 // Instruction descriptor, kind::i8: signed 8-bit operands, K-major, 32-bit integer sums.
@@ -299,47 +331,52 @@ __device__ __forceinline__ void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint
       : "memory");
 }
 
-template <typename T, bool TOKENS_A>
+template <typename T, bool TOKENS_A, bool STAGED>
 __global__ void __launch_bounds__(kI8Threads, 1)
-    i8_gemm_kernel(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUtensorMap mB, I8GemmArgs p) {
+    i8_gemm_kernel(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUtensorMap mB,
+                   const __grid_constant__ CUtensorMap mY, I8GemmArgs p) {
   extern __shared__ uint8_t i8_raw[];
   __shared__ I8Shared sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* ringA = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(i8_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* ringB = ringA + (size_t)p.stages * (kI8BM * kI8BK);
   const int b_bytes = p.bn * kI8BK;
-  const uint32_t tmem_cols = (uint32_t)(2 * p.bn);
+  uint8_t* stage = ringB + (size_t)p.stages * b_bytes;
+  const uint32_t tmem_cols = (uint32_t)(p.accs * p.bn);
   if (warp == 1) tmem_alloc(&sh.tmem_base, tmem_cols);
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < p.accs; ++i) {
       mbar_init(&sh.tfull[i], 1);
-      mbar_init(&sh.tempty[i], kI8EpiWarps * 32);
+      mbar_init(&sh.tempty[i], kI8EpiWarps * (p.share ? 32 : 16));
     }
     mbar_init(&sh.drain, 1);
     sh.abort = 0;
     fence_mbarrier_init();
     tma_prefetch_map(&mA);
     tma_prefetch_map(&mB);
+    if (STAGED) tma_prefetch_map(&mY);
   }
   if (warp == 1) tmem_relinquish();
+  grid_dependency_wait();  // the set-up above passes under the quantisation's end
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem_base;
   volatile int* abort = &sh.abort;
-  const int tiles = p.a_tiles * p.b_tiles;
+  const int tiles = p.a_tiles * p.samples * p.b_tiles;
   const int mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
   const int kblocks = (p.K + kI8BK - 1) / kI8BK;
   long long issued = 0;
   // neighbouring CTAs share a tile of tokens and differ in the output channels
-  const auto decode = [&](int i, int& a0, int& b0) {
-    const int t = (int)blockIdx.x + i * (int)gridDim.x;
-    const int ta = TOKENS_A ? t / p.b_tiles : t % p.a_tiles, tb = TOKENS_A ? t % p.b_tiles : t / p.a_tiles;
-    a0 = ta * kI8BM;
+  const auto decode = [&](int i, int& sample, int& a0, int& b0) {
+    const int t = (int)blockIdx.x + i * (int)gridDim.x, all = p.a_tiles * p.samples;
+    const int ta = TOKENS_A ? t / p.b_tiles : t % all, tb = TOKENS_A ? t % p.b_tiles : t / all;
+    sample = ta / p.a_tiles;
+    a0 = (ta - sample * p.a_tiles) * kI8BM;
     b0 = tb * p.bn;
   };
 
@@ -347,15 +384,15 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     if (lane == 0) {
       bool ok = true;
       for (int i = 0; i < mine && ok; ++i) {
-        int a0, b0;
-        decode(i, a0, b0);
+        int sample, a0, b0;
+        decode(i, sample, a0, b0);
         for (int kb = 0; kb < kblocks; ++kb) {
           const int st = (int)(issued % p.stages);
           const long long turn = issued / p.stages;
           if (turn > 0 && !(ok = wait_or_abort(&sh.empty[st], (uint32_t)((turn - 1) & 1), abort))) break;
           mbar_arrive_expect_tx(&sh.full[st], (uint32_t)(kI8BM * kI8BK + b_bytes));
-          tma_load_2d(ringA + (size_t)st * (kI8BM * kI8BK), &mA, &sh.full[st], kb * kI8BK, a0);
-          tma_load_2d(ringB + (size_t)st * b_bytes, &mB, &sh.full[st], kb * kI8BK, b0);
+          tma_load_3d(ringA + (size_t)st * (kI8BM * kI8BK), &mA, &sh.full[st], kb * kI8BK, a0, sample);
+          tma_load_3d(ringB + (size_t)st * b_bytes, &mB, &sh.full[st], kb * kI8BK, b0, 0);
           ++issued;
         }
       }
@@ -366,8 +403,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       long long q = 0;
       bool ok = true;
       for (int i = 0; i < mine && ok; ++i) {
-        const int acc = i & 1;
-        if (i >= 2 && !wait_or_abort(&sh.tempty[acc], (uint32_t)(((i >> 1) - 1) & 1), abort)) break;
+        const int acc = i % p.accs, turn = i / p.accs;
+        if (turn > 0 && !wait_or_abort(&sh.tempty[acc], (uint32_t)((turn - 1) & 1), abort)) break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(acc * p.bn);
         for (int kb = 0; kb < kblocks; ++kb, ++q) {
@@ -385,56 +422,123 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       }
     }
   } else {
-    // accumulator lanes 32 * (warp % 4) ..; the two groups of four warps take turns at the
-    // 32-column pieces
+    // accumulator lanes 32 * (warp % 4) ..; 32 columns at a time
     const int q4 = warp & 3, half = (warp - 2) >> 2;
-    float2* col = sh.col[warp - 2];
-    for (int i = 0; i < mine; ++i) {
-      const int acc = i & 1;
-      if (!__all_sync(0xffffffffu, wait_or_abort(&sh.tfull[acc], (uint32_t)((i >> 1) & 1), abort))) break;
-      tc_fence_after();
-      int a0, b0;
-      decode(i, a0, b0);
-      const int row = a0 + q4 * 32 + lane;
-      const bool in = row < p.a_rows;
-      float row_scale = 0.f, row_bias = 0.f;
-      T* y = static_cast<T*>(p.y);
-      long long step;  // from one column to the next
-      if (in) row_scale = p.a_scale[row];
-      if (TOKENS_A) {
-        const int o = row / p.inner;
-        y += ((long long)o * p.N + b0) * p.inner + (row - o * p.inner);
-        step = p.inner;
-      } else {
-        if (in && p.bias != nullptr) row_bias = p.bias[row];
-        y += (long long)b0 * p.N + row;
-        step = p.N;
-      }
-      for (int c0 = half * 32; c0 < p.bn && b0 + c0 < p.b_rows; c0 += 64) {
+    const int first = p.share ? half * 32 : 0, next = p.share ? 64 : 32;
+    float2* col = reinterpret_cast<float2*>(sh.col[warp - 2]);
+    uint8_t* stg = stage + (warp - 2) * 2 * kI8StageBytes;
+    int stored = 0;
+    for (int i = p.share ? 0 : half; i < mine; i += p.share ? 1 : 2) {
+      const int acc = i % p.accs;
+      int sample, a0, b0;
+      decode(i, sample, a0, b0);
+      const int r0 = a0 + q4 * 32;  // this warp's first row of A
+      const float* a_scale = p.a_scale + (long long)sample * p.a_rows;
+      // the constants of a column's output channel or token, shared by the warp's lanes
+      const auto columns = [&](int c0) {
         const int c = b0 + c0 + lane;
-        uint32_t r[32];
-        __syncwarp();  // whole again, and the previous piece's constants are read
-        tmem_ld32(tmem + (uint32_t)(acc * p.bn + c0) + ((uint32_t)(q4 * 32) << 16), r);
         col[lane] = c < p.b_rows ? make_float2(p.b_scale[c], TOKENS_A && p.bias != nullptr ? p.bias[c] : 0.f)
                                  : make_float2(0.f, 0.f);
-        __syncwarp();
-        tmem_ld_wait();
-        T* at = y + c0 * step;
-        const int n = min(32, p.b_rows - b0 - c0);
+      };
+      // (false: a wait ran out, the warp leaves)
+      const auto accumulated = [&] {
+        if (!__all_sync(0xffffffffu, wait_or_abort(&sh.tfull[acc], (uint32_t)((i / p.accs) & 1), abort))) return false;
+        tc_fence_after();
+        return true;
+      };
+      const uint32_t t0 = tmem + (uint32_t)(acc * p.bn) + ((uint32_t)(q4 * 32) << 16);
+      if constexpr (STAGED) {
+        // fragment layout: thread t has rows t / 4 + 8 i (i < 4) and column pairs 8 x + 2 (t % 4)
+        const int tr = lane >> 2, tc = lane & 3;
+        float2 rs[4];  // (scale, bias) of the rows
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float2 k = col[j];
-          const float v = (float)(int)r[j];
-          // (sum * token's scale) * channel's scale + bias
-          if (in && j < n)
-            *at = from_acc<T>(TOKENS_A ? fmaf(v * row_scale, k.x, k.y) : fmaf(v * k.x, row_scale, row_bias));
-          at += step;
+        for (int k = 0; k < 4; ++k) {
+          const int row = r0 + tr + 8 * k;
+          rs[k] = row < p.a_rows ? make_float2(a_scale[row], !TOKENS_A && p.bias != nullptr ? p.bias[row] : 0.f)
+                                 : make_float2(0.f, 0.f);
+        }
+        __syncwarp();
+        columns(first);  // like the rows' constants, on their way while the product is computed
+        if (!accumulated()) break;
+        for (int c0 = first; c0 < p.bn && b0 + c0 < p.b_rows; c0 += next) {
+          uint32_t r[2][2][8];  // [16 rows][16 columns]
+          __syncwarp();         // the previous piece's constants are read
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              tmem_ld_16x256b_x2(t0 + (uint32_t)(c0 + 16 * x) + ((uint32_t)(16 * h) << 16), r[h][x]);
+          if (c0 > first) columns(c0);
+          uint8_t* buf = stg + (stored & 1) * kI8StageBytes;
+          if (stored >= 2 && lane == 0) bulk_wait_read<1>();  // the store from this buffer has read it
+          __syncwarp();
+          tmem_ld_wait();
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float4 k[2];  // (scale, bias) x 2 of the columns 16 x + 8 y + 2 tc
+#pragma unroll
+            for (int y = 0; y < 2; ++y) k[y] = sh.col[warp - 2][8 * x + 4 * y + tc];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t q[4];
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {  // rows + 8 (m % 2), columns + 8 (m / 2)
+                const float2 v = make_float2((float)(int)r[h][x][2 * m], (float)(int)r[h][x][2 * m + 1]);
+                const float2 row = rs[2 * h + (m & 1)];
+                const float4 kc = k[m >> 1];
+                // (sum * token's scale) * channel's scale + bias
+                const float2 out =
+                    TOKENS_A ? __ffma2_rn(__fmul2_rn(v, make_float2(row.x, row.x)), make_float2(kc.x, kc.z), make_float2(kc.y, kc.w))
+                             : __ffma2_rn(__fmul2_rn(v, make_float2(kc.x, kc.z)), make_float2(row.x, row.x), make_float2(row.y, row.y));
+                q[m] = pack2<T>(out);
+              }
+              const int R = 16 * x + 8 * (lane >> 4) + (lane & 7);  // the column this lane addresses
+              const int u = 2 * h + ((lane >> 3) & 1);              // its 16 bytes: 8 rows of A
+              stsm_x4_trans(smem_u32(buf) + (uint32_t)(R * 64 + (((u ^ (R >> 1)) & 3) << 4)), q);
+            }
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0 && r0 < p.a_rows) {
+            if (TOKENS_A) tma_store_3d(&mY, buf, r0, b0 + c0, sample);
+            else tma_store_3d(&mY, buf, r0, b0 + c0, 0);
+          }
+          if (lane == 0) bulk_commit();
+          ++stored;
+        }
+      } else {
+        const int row = r0 + lane;
+        const bool in = row < p.a_rows;
+        const float row_scale = in ? a_scale[row] : 0.f;
+        const float row_bias = !TOKENS_A && in && p.bias != nullptr ? p.bias[row] : 0.f;
+        const long long step = TOKENS_A ? p.a_rows : p.N;  // of y, from one column to the next
+        T* y = static_cast<T*>(p.y) + row +
+               (TOKENS_A ? ((long long)sample * p.N + b0) * p.a_rows : (long long)b0 * p.N);
+        if (!accumulated()) break;
+        for (int c0 = first; c0 < p.bn && b0 + c0 < p.b_rows; c0 += next) {
+          uint32_t r[32];
+          __syncwarp();  // whole again, and the previous piece's constants are read
+          tmem_ld32(t0 + (uint32_t)c0, r);
+          columns(c0);
+          __syncwarp();
+          tmem_ld_wait();
+          T* at = y + c0 * step;
+          const int n = min(32, p.b_rows - b0 - c0);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float2 k = col[j];
+            const float v = (float)(int)r[j];
+            if (in && j < n)
+              *at = from_acc<T>(TOKENS_A ? fmaf(v * row_scale, k.x, k.y) : fmaf(v * k.x, row_scale, row_bias));
+            at += step;
+          }
         }
       }
       __syncwarp();
       tc_fence_before();
       mbar_arrive(&sh.tempty[acc]);
     }
+    if (STAGED && lane == 0) bulk_wait_all();
   }
   __syncthreads();
   if (*abort && lane == 0) {
@@ -450,7 +554,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 // Channels first with weights that stay in shared memory: the product is bound by the
 // bytes of x and y, so x is read, quantised, multiplied and written by the same CTA, and
 // no 8-bit rows go through memory (the two-kernel form reads and writes K bytes per token
-// more, and its accumulators pass through TMEM: 248 us against this kernel's TIMES us for
+// more, and its accumulators pass through TMEM: 248 us against this kernel's 84 us for
 // 32 -> 64 channels at 128^3, where x and y take 62 us of bandwidth).
 //
 // A tile is 32 W tokens.  Warp s of S = ceil(K / 32) quantises channels 32 s .. of it as
@@ -458,7 +562,11 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 // output channels, 16 at a time: mma.sync m16n8k32 with the weights as A, so that sums stay
 // in the registers of the thread that stores them.  Column n of the four B fragments of 32
 // tokens is token 8 (n / 2) + 2 j + n % 2 of them: a thread's columns 2 t, 2 t + 1 of
-// fragments j = 0 .. 3 are 8 neighbouring tokens, one 16-byte store of 16-bit data.
+// fragments j = 0 .. 3 are 8 neighbouring tokens, 16 bytes of 16-bit data.  A warp's
+// channels (up to 64) x the tile's 128 bytes of tokens go through shared memory and leave in
+// one TMA store where y's rows are whole 16-byte units: stored directly, a warp's 16-byte pieces
+// in 8 rows keep the L1 data pipe busy (74 %, the bound), and in many small TMA stores (16
+// channels x 64 bytes) their issue is the bound.
 __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -480,36 +588,57 @@ struct I8NarrowArgs {
   void* y;
   long long w_pitch;
   int outer, inner, K, N;
-  int vec;  // y's rows start on 16 bytes: 8 tokens per store
+  int mt_warp, mt_store;  // 16-channel pieces per warp, and per store (a divisor)
 };
 
-// Shared memory: weights [N16][row], per output channel (scale, bias), then per tile of the
-// CTA: token rows [32 W][row], their scales, and the warps' maxima [S][W][32].  row = K
-// rounded up to 32, plus 16: an odd number of 16-byte units, so that eight rows' ldmatrix
-// reads fall on different banks.
+// Shared memory: a staging buffer per warp, weights [N16][row], per output channel (scale,
+// bias), then per tile of the CTA: token rows [32 W][row], their scales, and the warps' maxima
+// [S][W][32].  row = K
+// rounded up to 32, plus 16: an odd number of 16-byte units, so that eight neighbouring rows'
+// ldmatrix reads fall on different banks; eight tokens' rows take 32 bytes more, which does
+// the same for the permuted tokens of a B fragment.
 __host__ __device__ __forceinline__ int narrow_row(int K) { return (K + 31) / 32 * 32 + 16; }
+__host__ __device__ __forceinline__ int narrow_token(int t, int row) { return t * row + (t >> 3) * 32; }
 __host__ __device__ __forceinline__ int narrow_tile_bytes(int K, int W) {
-  return 32 * W * narrow_row(K) + 32 * W * 4 + (K + 31) / 32 * W * 128;
+  return narrow_token(32 * W, narrow_row(K)) + 32 * W * 4 + (K + 31) / 32 * W * 128;
 }
 __host__ __device__ __forceinline__ int narrow_weight_bytes(int K, int N) {
   return (N + 15) / 16 * 16 * (narrow_row(K) + 8);
 }
 
-template <typename T, int W>
-__global__ void __launch_bounds__(512) i8_narrow_kernel(I8NarrowArgs a) {
-  extern __shared__ __align__(16) uint8_t i8_sm[];
-  const int lane = threadIdx.x, s = threadIdx.y, S = blockDim.y, P = blockDim.z;
+// Bytes of staging per 16 channels: 128-byte rows (64 tokens of 16-bit data, 32 of fp32),
+// 128-byte swizzle.
+constexpr int kNarrowStage = 16 * 128;
+constexpr int kNarrowMtStore = 2;
+constexpr int kNarrowWarps = 16;  // resident per SM, at 128 registers
+template <typename T>
+constexpr int kNarrowW = 4 / (int)sizeof(T);  // tokens per lane
+
+// S = KB = ceil(K / 32) is 1 or 2: a tile's B fragments stay in registers over the output
+// channels.  The sums are below 2^22, so they start from the bits of 1.5 * 2^23 and are the
+// mantissa of a float already: a subtraction takes the place of the conversion, which runs
+// at an eighth of the rate.
+constexpr int kSumBits = 0x4B400000;
+
+template <typename T, int KB>
+__global__ void __launch_bounds__(kNarrowWarps * 32, 1)
+    i8_narrow_kernel(const __grid_constant__ CUtensorMap mY, I8NarrowArgs a) {
+  constexpr int W = kNarrowW<T>, S = KB;
+  extern __shared__ uint8_t i8_raw[];
+  const int lane = threadIdx.x, s = threadIdx.y, P = blockDim.z;
   const int row = narrow_row(a.K), n16 = (a.N + 15) / 16;
-  uint8_t* wsm = i8_sm;
-  float2* chan = reinterpret_cast<float2*>(i8_sm + n16 * 16 * row);
-  uint8_t* tile_sm = i8_sm + narrow_weight_bytes(a.K, a.N) + threadIdx.z * narrow_tile_bytes(a.K, W);
-  float* tscale = reinterpret_cast<float*>(tile_sm + 32 * W * row);
+  uint8_t* base_sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(i8_raw) + 1023) & ~(uintptr_t)1023);
+  const int stage_bytes = a.mt_store * kNarrowStage;
+  uint8_t* stg = base_sm + (s + S * threadIdx.z) * stage_bytes;
+  uint8_t* wsm = base_sm + S * P * stage_bytes;
+  float2* chan = reinterpret_cast<float2*>(wsm + n16 * 16 * row);
+  uint8_t* tile_sm = wsm + narrow_weight_bytes(a.K, a.N) + threadIdx.z * narrow_tile_bytes(a.K, W);
+  float* tscale = reinterpret_cast<float*>(tile_sm + narrow_token(32 * W, row));
   uint32_t* maxima = reinterpret_cast<uint32_t*>(tscale + 32 * W);
   {
     const int me = threadIdx.x + 32 * (threadIdx.y + S * threadIdx.z), all = 32 * S * P;
-    const int pieces = (row - 16) / 16;
-    for (int i = me; i < n16 * 16 * pieces; i += all) {
-      const int n = i / pieces, k = (i - n * pieces) * 16;
+    for (int i = me; i < n16 * 16 * 2 * KB; i += all) {
+      const int n = i / (2 * KB), k = (i - n * (2 * KB)) * 16;
       uint4 v = make_uint4(0, 0, 0, 0);
       // the last 16 bytes of a row may hold bytes past K: they meet zeros of x
       if (n < a.N && k < a.K) v = *reinterpret_cast<const uint4*>(a.w + n * a.w_pitch + k);
@@ -519,8 +648,9 @@ __global__ void __launch_bounds__(512) i8_narrow_kernel(I8NarrowArgs a) {
       chan[n] = n < a.N ? make_float2(a.ws[n], a.bias != nullptr ? a.bias[n] : 0.f) : make_float2(0.f, 0.f);
   }
   __syncthreads();
+  // the warps of a tile meet at a barrier of their own
   const auto meet = [&] {
-    if (S > 1) __syncthreads();
+    if (S > 1) asm volatile("bar.sync %0, %1;" ::"r"((int)threadIdx.z + 1), "n"(32 * S) : "memory");
     else __syncwarp();
   };
   const int per = (a.inner + 32 * W - 1) / (32 * W);
@@ -531,37 +661,35 @@ __global__ void __launch_bounds__(512) i8_narrow_kernel(I8NarrowArgs a) {
   // B takes fragment j's two halves, then fragment j + 1's, rows being the permuted tokens
   const uint32_t a_off = (uint32_t)((lane & 15) * row + (lane >> 4) * 16);
   const int bn = lane & 7;
-  const uint32_t b_off = (uint32_t)((8 * (bn >> 1) + 2 * (lane >> 4) + (bn & 1)) * row + ((lane >> 3) & 1) * 16);
-  for (long long base = (long long)blockIdx.x * P; base < tiles; base += (long long)gridDim.x * P) {
-    const long long tile = base + threadIdx.z;
-    const int o = (int)(tile / per), v0 = (int)(tile - (long long)o * per) * (32 * W), v = v0 + lane * W;
-    const bool in = tile < tiles && v < a.inner;  // inner is even where W = 2
+  const uint32_t b_off = (uint32_t)(narrow_token(8 * (bn >> 1) + 2 * (lane >> 4) + (bn & 1), row) + ((lane >> 3) & 1) * 16);
+  const int mine = min(32, a.K - s * 32), mt_end = min(n16, (s + 1) * a.mt_warp);
+  uint32_t x[32];
+  // the tile's x: of the first before the loop, of each next one as soon as the last is
+  // quantised, so that its loads pass under the products and the stores
+  const auto load = [&](long long tile) {
+    const int o = (int)(tile / per), v = (int)(tile - (long long)o * per) * (32 * W) + lane * W;
+    const bool in = tile < tiles && v < a.inner;  // inner is a multiple of W
     const T* px = static_cast<const T*>(a.x) + ((long long)o * a.K + s * 32) * a.inner + v;
-    const int mine = min(32, a.K - s * 32);
-    uint32_t x[32];
 #pragma unroll
     for (int k = 0; k < 32; ++k) {
-      const bool ok = in && k < mine;
-      if constexpr (W == 2) x[k] = ok ? *reinterpret_cast<const uint32_t*>(px) : 0u;
-      else if constexpr (sizeof(T) == 4) x[k] = ok ? __float_as_uint(*px) : 0u;
-      else x[k] = ok ? (uint32_t)*reinterpret_cast<const uint16_t*>(px) : 0u;
+      x[k] = in && k < mine ? *reinterpret_cast<const uint32_t*>(px) : 0u;
       px += a.inner;
       asm volatile("" : "+l"(px));  // one address in flight, not 32
     }
+  };
+  load((long long)blockIdx.x * P + threadIdx.z);
+  for (long long base = (long long)blockIdx.x * P; base < tiles; base += (long long)gridDim.x * P) {
+    const long long tile = base + threadIdx.z;
+    const int o = (int)(tile / per), v0 = (int)(tile - (long long)o * per) * (32 * W);
     uint32_t m = 0;
 #pragma unroll
-    for (int k = 0; k < 32; ++k) {
-      if constexpr (W == 2) m = __vmaxu2(m, x[k] & 0x7fff7fffu);
-      else m = max(m, x[k] & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fffu));
-    }
+    for (int k = 0; k < 32; ++k) m = W == 2 ? __vmaxu2(m, x[k] & 0x7fff7fffu) : max(m, x[k] & 0x7fffffffu);
     uint32_t most[W];
     if constexpr (W == 2) {
       most[0] = Mag<T>::lo(m);
-      most[W - 1] = Mag<T>::hi(m);
-    } else if constexpr (sizeof(T) == 4) {
-      most[0] = m;
+      most[1] = Mag<T>::hi(m);
     } else {
-      most[0] = abs_bits(unpack2<T>(m).x);
+      most[0] = m;
     }
     if (S > 1) {
 #pragma unroll
@@ -570,8 +698,7 @@ __global__ void __launch_bounds__(512) i8_narrow_kernel(I8NarrowArgs a) {
     meet();  // the maxima are there, and the last tile's rows are read
     if (S > 1) {
 #pragma unroll
-      for (int j = 0; j < W; ++j)
-        for (int i = 0; i < S; ++i) most[j] = max(most[j], maxima[(i * W + j) * 32 + lane]);
+      for (int j = 0; j < W; ++j) most[j] = max(maxima[j * 32 + lane], maxima[(W + j) * 32 + lane]);
     }
     TokenScale ts[W];
 #pragma unroll
@@ -582,75 +709,205 @@ __global__ void __launch_bounds__(512) i8_narrow_kernel(I8NarrowArgs a) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t b[W][4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float2 f[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t word = x[h * 16 + i * 4 + e];
-          if constexpr (W == 2) f[e] = unpack2<T>(word);
-          else if constexpr (sizeof(T) == 4) f[e] = make_float2(__uint_as_float(word), 0.f);
-          else f[e] = make_float2(unpack2<T>(word).x, 0.f);
-          f[e] = scaled2(f[e], ts[0].inverse, ts[W - 1].inverse);
-        }
-        b[0][i] = low_bytes(f[0].x, f[1].x, f[2].x, f[3].x);
-        if constexpr (W == 2) b[1][i] = low_bytes(f[0].y, f[1].y, f[2].y, f[3].y);
-      }
+      quantize16<T, W>(x + h * 16, ts, b);
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         const uint32_t keep = most[j] >= 0x7f800000u ? 0u : 0xffffffffu;
-        *reinterpret_cast<uint4*>(tile_sm + (lane * W + j) * row + s * 32 + h * 16) =
+        *reinterpret_cast<uint4*>(tile_sm + narrow_token(lane * W + j, row) + s * 32 + h * 16) =
             make_uint4(b[j][0] & keep, b[j][1] & keep, b[j][2] & keep, b[j][3] & keep);
       }
     }
     meet();
-    if (tile < tiles) {
+    if (base + (long long)gridDim.x * P < tiles) load(tile + (long long)gridDim.x * P);
+#pragma unroll 1
+    for (int mt0 = s * a.mt_warp; tile < tiles && mt0 < mt_end; mt0 += a.mt_store) {
+      if (lane == 0) bulk_wait_read<0>();  // the last store has read the buffer
+      __syncwarp();
 #pragma unroll 1
       for (int part = 0; part < W; ++part) {  // 32 tokens at a time
-        const int tok = part * 32 + 8 * t4, vt = v0 + tok;
-        float sc[8];
+        const int tok = part * 32 + 8 * t4;
+        const uint32_t b_addr = t_addr + (uint32_t)narrow_token(part * 32, row) + b_off;
+        const float4 lo = *reinterpret_cast<const float4*>(tscale + tok);
+        const float4 hi = *reinterpret_cast<const float4*>(tscale + tok + 4);
+        const float2 sc[4] = {make_float2(lo.x, lo.y), make_float2(lo.z, lo.w), make_float2(hi.x, hi.y),
+                              make_float2(hi.z, hi.w)};
+        uint32_t fb[KB][2][4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sc[i] = tscale[tok + i];
+        for (int kb = 0; kb < KB; ++kb) {
+          ldsm_x4(b_addr + kb * 32, fb[kb][0]);
+          ldsm_x4(b_addr + (uint32_t)(4 * row) + kb * 32, fb[kb][1]);
+        }
 #pragma unroll 1
-        for (int mt = s; mt < n16; mt += S) {
-          int acc[4][4] = {};
-          for (int kb = 0; kb < row - 16; kb += 32) {
-            uint32_t fa[4], fb[2][4];
-            ldsm_x4(w_addr + (uint32_t)(mt * 16 * row + kb) + a_off, fa);
-            ldsm_x4(t_addr + (uint32_t)(part * 32 * row + kb) + b_off, fb[0]);
-            ldsm_x4(t_addr + (uint32_t)((part * 32 + 4) * row + kb) + b_off, fb[1]);
+        for (int mt = mt0; mt < min(mt_end, mt0 + a.mt_store); ++mt) {
+          int acc[4][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mma_s8(acc[j], fa, fb[j >> 1][(j & 1) * 2], fb[j >> 1][(j & 1) * 2 + 1]);
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[j][i] = kSumBits;
+          const uint32_t a_addr = w_addr + (uint32_t)(mt * 16 * row) + a_off;
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+            uint32_t fa[4];
+            ldsm_x4(a_addr + kb * 32, fa);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma_s8(acc[j], fa, fb[kb][j >> 1][(j & 1) * 2], fb[kb][j >> 1][(j & 1) * 2 + 1]);
           }
+          uint8_t* buf = stg + (mt - mt0) * kNarrowStage;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {  // channels g and g + 8
-            const int n = mt * 16 + h * 8 + g;
-            if (n >= a.N) continue;
-            const float2 c = chan[n];
-            float out[8];
+            const int r = h * 8 + g;
+            const float2 c = chan[mt * 16 + r];  // zeros past N
+            float2 out[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) out[i] = fmaf((float)acc[i >> 1][h * 2 + (i & 1)] * sc[i], c.x, c.y);
-            T* y = static_cast<T*>(a.y) + ((long long)o * a.N + n) * a.inner + vt;
-            if (a.vec && vt + 8 <= a.inner) {
-              constexpr int E = 16 / sizeof(T);
-#pragma unroll
-              for (int i = 0; i < 8; i += E) *reinterpret_cast<uint4*>(y + i) = pack16<T>(out + i);
+            for (int j = 0; j < 4; ++j) {
+              const float2 v = __fadd2_rn(make_float2(__int_as_float(acc[j][h * 2]), __int_as_float(acc[j][h * 2 + 1])),
+                                          make_float2(-kRint, -kRint));
+              out[j] = __ffma2_rn(__fmul2_rn(v, sc[j]), make_float2(c.x, c.x), make_float2(c.y, c.y));
+            }
+            const float* f = reinterpret_cast<const float*>(out);
+            if constexpr (W == 2) {
+              *reinterpret_cast<uint4*>(buf + r * 128 + (((part * 4 + t4) ^ (r & 7)) << 4)) = pack16<T>(f);
             } else {
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (vt + i < a.inner) y[i] = from_acc<T>(out[i]);
+              *reinterpret_cast<uint4*>(buf + r * 128 + (((2 * t4) ^ (r & 7)) << 4)) = pack16<T>(f);
+              *reinterpret_cast<uint4*>(buf + r * 128 + (((2 * t4 + 1) ^ (r & 7)) << 4)) = pack16<T>(f + 4);
             }
           }
         }
       }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(&mY, stg, v0, mt0 * 16, o);
+        bulk_commit();
+      }
+    }
+  }
+  if (lane == 0) bulk_wait_all();
+}
+
+// 16-channel pieces per warp and per store: the most, up to kNarrowMtStore, that divide a warp's share
+// (a store's box may not reach into the next warp's channels).
+void narrow_share(int N, int S, int* mt_warp, int* mt_store) {
+  *mt_warp = ((N + 15) / 16 + S - 1) / S;
+  *mt_store = kNarrowMtStore;
+  while (*mt_warp % *mt_store != 0) --*mt_store;
+}
+// Shared memory of a CTA of P tiles.
+size_t narrow_smem(int K, int N, int W, int P) {
+  const int S = (K + 31) / 32;
+  int mt_warp, mt_store;
+  narrow_share(N, S, &mt_warp, &mt_store);
+  return (size_t)narrow_weight_bytes(K, N) + (size_t)P * (narrow_tile_bytes(K, W) + S * mt_store * kNarrowStage) + 1024;
+}
+// Whether the one-kernel form takes a product: K and N small enough that bytes are its bound
+// (bf16, 64^3 voxels: 64 -> 192 channels 48 us against 51 us in two kernels, but 192 -> 64
+// 65 us against 64, 128 -> 512 34 against 22), whole 16-byte rows, and enough tiles.
+bool narrow_takes(const void* x, const void* y, long long outer, int K, long long inner, int N, size_t esz) {
+  return K <= 64 && N <= 256 && inner % (16 / (long long)esz) == 0 && reinterpret_cast<uintptr_t>(x) % 4 == 0 &&
+         reinterpret_cast<uintptr_t>(y) % 16 == 0 && outer * ((inner + 63) / 64) >= 2 * kI8Sms;
+}
+
+// ------------------------------ a few tokens ------------------------------
+// Up to eight tokens: the weights' bytes and the launch count, not the tokens.  One kernel:
+// a warp owns one output channel and asks for the first 2 KB of its weights before anything
+// else; meanwhile the CTA quantises all tokens into shared memory (each CTA for itself: they
+// are a few KB, from L2).  Then dot products of four bytes a lane, and a warp sum.
+// One token 512 -> 2048: 3.9 us; as two kernels 8.3 us.
+constexpr int kI8FewTokens = 8, kI8FewWarps = 8;
+
+struct I8FewArgs {
+  const void* x;
+  const int8_t* w;
+  const float* ws;
+  const float* bias;  // or NULL
+  void* y;
+  long long w_pitch;
+  int tokens, inner, K, N;
+  int per_token;  // warps that quantise a token
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kI8FewWarps * 32) i8_few_kernel(I8FewArgs a) {
+  extern __shared__ __align__(16) uint8_t i8_few[];  // [tokens][K rounded up to 16]
+  __shared__ uint32_t most[kI8FewWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = blockIdx.x * kI8FewWarps + warp;
+  const int row = (a.K + 15) / 16 * 16, chunks = row / 16;
+  const uint4* w = reinterpret_cast<const uint4*>(a.w + (long long)n * a.w_pitch);
+  uint4 ahead[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    ahead[i] = n < a.N && lane + 32 * i < chunks ? w[lane + 32 * i] : make_uint4(0, 0, 0, 0);
+  // four values per lane and turn
+  const int token = warp / a.per_token, part = warp - token * a.per_token;
+  const int o = token / a.inner;
+  const T* x = static_cast<const T*>(a.x) + (long long)o * a.K * a.inner + (token - o * a.inner);
+  const auto value = [&](int k) { return k < a.K ? to_acc<T>(x[(long long)k * a.inner]) : 0.f; };
+  uint32_t m = 0;
+  if (token < a.tokens)
+    for (int k = (part * 32 + lane) * 4; k < a.K; k += a.per_token * 128) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = max(m, abs_bits(value(k + e)));
+    }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (lane == 0) most[warp] = m;
+  __syncthreads();
+  if (token < a.tokens) {
+    for (int i = 0; i < a.per_token; ++i) m = max(m, most[token * a.per_token + i]);
+    const TokenScale ts = token_scale(m);
+    const uint32_t keep = m >= 0x7f800000u ? 0u : 0xffffffffu;
+    for (int k = (part * 32 + lane) * 4; k < row; k += a.per_token * 128) {
+      const float2 f = scaled2(make_float2(value(k), value(k + 1)), ts.inverse, ts.inverse);
+      const float2 g = scaled2(make_float2(value(k + 2), value(k + 3)), ts.inverse, ts.inverse);
+      *reinterpret_cast<uint32_t*>(i8_few + token * row + k) = low_bytes(f.x, f.y, g.x, g.y) & keep;
+    }
+  }
+  __syncthreads();
+  if (n >= a.N) return;
+  int acc[kI8FewTokens] = {};
+  const auto dot = [&](const uint4& v, int c) {
+#pragma unroll
+    for (int t = 0; t < kI8FewTokens; ++t) {
+      if (t >= a.tokens) break;
+      const uint4 u = *reinterpret_cast<const uint4*>(i8_few + t * row + c * 16);
+      acc[t] = __dp4a((int)v.x, (int)u.x, acc[t]);
+      acc[t] = __dp4a((int)v.y, (int)u.y, acc[t]);
+      acc[t] = __dp4a((int)v.z, (int)u.z, acc[t]);
+      acc[t] = __dp4a((int)v.w, (int)u.w, acc[t]);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane + 32 * i < chunks) dot(ahead[i], lane + 32 * i);
+  for (int c = lane + 128; c < chunks; c += 32) dot(w[c], c);
+  const float scale = a.ws[n], bias = a.bias != nullptr ? a.bias[n] : 0.f;
+#pragma unroll
+  for (int t = 0; t < kI8FewTokens; ++t) {
+    if (t >= a.tokens) break;
+    const int sum = __reduce_add_sync(0xffffffffu, acc[t]);
+    if (lane == t) {
+      uint32_t mt = 0;
+      for (int i = 0; i < a.per_token; ++i) mt = max(mt, most[t * a.per_token + i]);
+      const int ot = t / a.inner;
+      static_cast<T*>(a.y)[((long long)ot * a.N + n) * a.inner + (t - ot * a.inner)] =
+          from_acc<T>(fmaf((float)sum * token_scale(mt).scale, scale, bias));
     }
   }
 }
 
-// Whether the one-kernel form covers K and N: its weights and one tile in 100 KB of shared
-// memory (two CTAs per SM), 16 warps.
-bool narrow_covers(int K, int N) {
-  return K <= 512 && narrow_weight_bytes(K, N) + narrow_tile_bytes(K, 2) <= 100 * 1024;
+// Whether the one-kernel form for a few tokens takes a product: its 8-bit rows fit.
+bool few_takes(long long tokens, int K) { return tokens <= kI8FewTokens && tokens * ((K + 15) / 16 * 16) <= 64 * 1024; }
+
+template <typename T>
+int launch_few(I8FewArgs a, cudaStream_t s) {
+  int tokens = 1;
+  while (tokens < a.tokens) tokens *= 2;
+  a.per_token = kI8FewWarps / tokens;
+  const size_t smem = (size_t)a.tokens * ((a.K + 15) / 16 * 16);
+  const int st = ensure_smem(i8_few_kernel<T>, smem);
+  if (st != MEDNEXT_OK) return st;
+  i8_few_kernel<T><<<(a.N + kI8FewWarps - 1) / kI8FewWarps, kI8FewWarps * 32, smem, s>>>(a);
+  return record_launch();
 }
 
 int num_sms() {
@@ -661,10 +918,10 @@ int num_sms() {
   return sms;
 }
 
-// q: [tokens][q_pitch], w: [N][w_pitch]; y [outer, N, inner]
+// q: [outer * inner][q_pitch], w: [N][w_pitch]; y [outer, N, inner]
 template <typename T>
 int launch_gemm(const int8_t* q, const float* qs, long long q_pitch, const int8_t* w, const float* ws,
-                long long w_pitch, const float* bias, void* y, long long tokens, long long inner, int K, int N,
+                long long w_pitch, const float* bias, void* y, long long outer, long long inner, int K, int N,
                 cudaStream_t s) {
   const bool tokens_a = inner > 1;
   I8GemmArgs p{};
@@ -672,35 +929,47 @@ int launch_gemm(const int8_t* q, const float* qs, long long q_pitch, const int8_
   p.b_scale = tokens_a ? ws : qs;
   p.bias = bias;
   p.y = y;
-  p.a_rows = tokens_a ? (int)tokens : N;
-  p.b_rows = tokens_a ? N : (int)tokens;
+  p.a_rows = tokens_a ? (int)inner : N;
+  p.samples = tokens_a ? (int)outer : 1;
+  p.b_rows = tokens_a ? N : (int)outer;
   p.K = K;
-  p.inner = (int)inner;
   p.N = N;
   p.a_tiles = (p.a_rows + kI8BM - 1) / kI8BM;
   const int sms = num_sms();
+  const long long a_all = (long long)p.a_tiles * p.samples;
   // the widest B tile that still gives every SM a tile, at most what B fills
   p.bn = 256;
-  while (p.bn > 32 && (p.bn / 2 >= p.b_rows || (long long)p.a_tiles * ((p.b_rows + p.bn - 1) / p.bn) < sms)) p.bn /= 2;
+  while (p.bn > 32 && (p.bn / 2 >= p.b_rows || a_all * ((p.b_rows + p.bn - 1) / p.bn) < sms)) p.bn /= 2;
   p.b_tiles = (p.b_rows + p.bn - 1) / p.bn;
-  if ((long long)p.a_tiles * p.b_tiles >= ((long long)1 << 31)) return MEDNEXT_ERR_BAD_SHAPE;
-  const int stage = kI8BM * kI8BK + p.bn * kI8BK;
-  p.stages = std::min(kI8MaxStages, (200 * 1024) / stage);
-  const size_t smem = (size_t)p.stages * stage + 1024;
-  CUtensorMap mA, mB;
-  if (!tma::encode_rows_8bit(&mA, tokens_a ? q : w, K, p.a_rows, tokens_a ? q_pitch : w_pitch, kI8BM) ||
-      !tma::encode_rows_8bit(&mB, tokens_a ? w : q, K, p.b_rows, tokens_a ? w_pitch : q_pitch, p.bn)) {
+  if (a_all * p.b_tiles >= ((long long)1 << 31)) return MEDNEXT_ERR_BAD_SHAPE;
+  p.accs = std::min(kI8MaxAcc, 512 / p.bn);
+  p.share = p.accs < 4 || a_all * p.b_tiles <= sms;
+  const int ring = kI8BM * kI8BK + p.bn * kI8BK, staging = kI8EpiWarps * 2 * kI8StageBytes;
+  p.stages = std::min(kI8MaxStages, (216 * 1024 - staging) / ring);
+  const size_t smem = (size_t)p.stages * ring + staging + 1024;
+  CUtensorMap mA, mB, mY;
+  memset(&mY, 0, sizeof(mY));
+  bool staged = false;
+  bool ok = tma::encode_rows_8bit(&mA, tokens_a ? q : w, K, p.a_rows, p.samples, tokens_a ? q_pitch : w_pitch, kI8BM) &&
+            tma::encode_rows_8bit(&mB, tokens_a ? w : q, K, p.b_rows, 1, tokens_a ? w_pitch : q_pitch, p.bn);
+  if constexpr (sizeof(T) == 2) {
+    staged = p.a_rows % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+    if (staged)
+      ok = ok && tma::encode3<T>(&mY, y, p.a_rows, p.b_rows, p.samples, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+  }
+  if (!ok) {
     note_cuda_error(cudaErrorInvalidValue);
     return MEDNEXT_ERR_CUDA;
   }
-  const unsigned grid = (unsigned)std::min<long long>((long long)p.a_tiles * p.b_tiles, sms);
+  const unsigned grid = (unsigned)std::min<long long>(a_all * p.b_tiles, sms);
   auto run = [&](auto kern) {
     const int st = ensure_smem(kern, smem);
     if (st != MEDNEXT_OK) return st;
-    kern<<<grid, kI8Threads, smem, s>>>(mA, mB, p);
-    return record_launch();
+    return launch_dependent(kern, dim3(grid), dim3(kI8Threads), smem, s, mA, mB, mY, p);
   };
-  return tokens_a ? run(i8_gemm_kernel<T, true>) : run(i8_gemm_kernel<T, false>);
+  if constexpr (sizeof(T) == 2)
+    if (staged) return tokens_a ? run(i8_gemm_kernel<T, true, true>) : run(i8_gemm_kernel<T, false, true>);
+  return tokens_a ? run(i8_gemm_kernel<T, true, false>) : run(i8_gemm_kernel<T, false, false>);
 }
 
 long long pitch16(int64_t k) { return (k + 15) / 16 * 16; }
@@ -711,20 +980,19 @@ int launch_quantize(const void* xv, int8_t* q, float* scale, long long outer, in
   const long long tokens = outer * inner;
   const T* x = static_cast<const T*>(xv);
   if (inner > 1) {
-    // two tokens per word where the alignment allows and the halved tiles still fill the GPU
-    const bool pair = sizeof(T) == 2 && inner % 2 == 0 && (reinterpret_cast<uintptr_t>(xv) & 3) == 0 &&
-                      outer * ((inner + 63) / 64) >= kI8Sms;
-    const int W = pair ? 2 : 1, S = std::min(32, (K + 31) / 32), P = std::max(1, 4 / S);
-    const long long tiles = outer * ((inner + 32 * W - 1) / (32 * W));
-    const unsigned grid = (unsigned)std::min<long long>((tiles + P - 1) / P, kI8Sms * 64);
-    const size_t smem = 2 * (size_t)P * S * W * 32 * sizeof(uint32_t);
+    const bool pair = sizeof(T) == 2 && inner % 2 == 0 && (reinterpret_cast<uintptr_t>(xv) & 3) == 0;
+    auto run = [&](auto kern, int W, int TX, int piece) {
+      const int S = (int)std::min<long long>(32, (pitch + piece - 1) / piece), P = std::max(1, 4 / S);
+      const long long tiles = outer * ((inner + TX * W - 1) / (TX * W));
+      const unsigned grid = (unsigned)std::min<long long>((tiles + P - 1) / P, kI8Sms * 64);
+      kern<<<grid, dim3(32, S, P), 2 * (size_t)P * S * W * TX * sizeof(uint32_t), s>>>(x, q, scale, (int)outer,
+                                                                                       (int)inner, K, (int)pitch);
+      return record_launch();
+    };
+    const bool few = outer * ((inner + 63) / 64) < kI8Sms;
     if constexpr (sizeof(T) == 2)
-      if (pair) {
-        i8_quantize_chan_kernel<T, 2><<<grid, dim3(32, S, P), smem, s>>>(x, q, scale, (int)outer, (int)inner, K, (int)pitch);
-        return record_launch();
-      }
-    i8_quantize_chan_kernel<T, 1><<<grid, dim3(32, S, P), smem, s>>>(x, q, scale, (int)outer, (int)inner, K, (int)pitch);
-    return record_launch();
+      if (pair) return few ? run(i8_quantize_chan_kernel<T, 2, 8, 16>, 2, 8, 64) : run(i8_quantize_chan_kernel<T, 2, 32, 32>, 2, 32, 32);
+    return few ? run(i8_quantize_chan_kernel<T, 1, 8, 16>, 1, 8, 64) : run(i8_quantize_chan_kernel<T, 1, 32, 32>, 1, 32, 32);
   }
   constexpr int E = 16 / sizeof(T);
   const int vecs = (int)((pitch + E - 1) / E);
@@ -745,42 +1013,49 @@ int launch_quantize(const void* xv, int8_t* q, float* scale, long long outer, in
 }
 
 template <typename T>
-int launch_narrow(const I8NarrowArgs& a, cudaStream_t s) {
-  const uintptr_t xb = reinterpret_cast<uintptr_t>(a.x);
-  const bool pair = sizeof(T) == 2 && a.inner % 2 == 0 && xb % 4 == 0;
-  const int W = pair ? 2 : 1, S = (a.K + 31) / 32;
-  int P = std::max(1, 4 / S);
-  while (P > 1 && narrow_weight_bytes(a.K, a.N) + P * narrow_tile_bytes(a.K, W) > 100 * 1024) --P;
-  const size_t smem = narrow_weight_bytes(a.K, a.N) + (size_t)P * narrow_tile_bytes(a.K, W);
+int launch_narrow(I8NarrowArgs a, cudaStream_t s) {
+  constexpr int W = kNarrowW<T>;
+  const int S = (a.K + 31) / 32, P = 4 / S;
+  const size_t smem = narrow_smem(a.K, a.N, W, P);
+  narrow_share(a.N, S, &a.mt_warp, &a.mt_store);
   const long long tiles = (long long)a.outer * ((a.inner + 32 * W - 1) / (32 * W));
-  // resident CTAs: 32 warps by registers, and what shared memory holds
-  const int per_sm = std::max(1, std::min(32 / (S * P), (int)(220 * 1024 / (smem + 1024))));
-  const unsigned grid = (unsigned)std::min<long long>((tiles + P - 1) / P, (long long)kI8Sms * per_sm);
+  // four turns of the resident CTAs, so that SMs that are done early take more
+  const int per_sm = std::max(1, std::min(kNarrowWarps / (S * P), (int)(227 * 1024 / (smem + 1024))));
+  const unsigned grid = (unsigned)std::min((tiles + P - 1) / P, 4LL * kI8Sms * per_sm);
+  CUtensorMap mY;
+  if (!tma::encode3<T>(&mY, a.y, a.inner, a.N, a.outer, 32 * W, 16 * a.mt_store, CU_TENSOR_MAP_SWIZZLE_128B)) {
+    note_cuda_error(cudaErrorInvalidValue);
+    return MEDNEXT_ERR_CUDA;
+  }
   auto run = [&](auto kern) {
     const int st = ensure_smem(kern, smem);
     if (st != MEDNEXT_OK) return st;
-    kern<<<grid, dim3(32, S, P), smem, s>>>(a);
+    kern<<<grid, dim3(32, S, P), smem, s>>>(mY, a);
     return record_launch();
   };
-  if constexpr (sizeof(T) == 2)
-    if (pair) return run(i8_narrow_kernel<T, 2>);
-  return run(i8_narrow_kernel<T, 1>);
+  return S == 1 ? run(i8_narrow_kernel<T, 1>) : run(i8_narrow_kernel<T, 2>);
 }
 
 template <typename T>
 int launch_linear(const void* x, const int8_t* w, const float* ws, long long w_pitch, const float* bias, void* y,
                   int8_t* q, float* qs, long long outer, int K, long long inner, int N, cudaStream_t s) {
-  if (inner > 1 && narrow_covers(K, N) && outer * ((inner + 63) / 64) >= kI8Sms) {
+  if (few_takes(outer * inner, K)) {
+    I8FewArgs a{};
+    a.x = x; a.w = w; a.ws = ws; a.bias = bias; a.y = y;
+    a.w_pitch = w_pitch;
+    a.tokens = (int)(outer * inner); a.inner = (int)inner; a.K = K; a.N = N;
+    return launch_few<T>(a, s);
+  }
+  if (inner > 1 && narrow_takes(x, y, outer, K, inner, N, sizeof(T))) {
     I8NarrowArgs a{};
     a.x = x; a.w = w; a.ws = ws; a.bias = bias; a.y = y;
     a.w_pitch = w_pitch;
     a.outer = (int)outer; a.inner = (int)inner; a.K = K; a.N = N;
-    a.vec = inner % (16 / (long long)sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
     return launch_narrow<T>(a, s);
   }
   int st = launch_quantize<T>(x, q, qs, outer, K, inner, pitch16(K), s);
   if (st != MEDNEXT_OK) return st;
-  return launch_gemm<T>(q, qs, pitch16(K), w, ws, w_pitch, bias, y, outer * inner, inner, K, N, s);
+  return launch_gemm<T>(q, qs, pitch16(K), w, ws, w_pitch, bias, y, outer, inner, K, N, s);
 }
 
 int i8_check(int64_t outer, int64_t k, int64_t inner, int dtype) {

@@ -244,6 +244,7 @@ __global__ void __launch_bounds__(1024) ln_fold_kernel(const float* __restrict__
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   double s0 = 0.0, s1 = 0.0;
+  grid_dependency_wait();
   if (c < C)
 #pragma unroll 8
     for (int p = warp; p < parts; p += 32) {
@@ -546,6 +547,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) ln_rows_bwd_kernel(LnArgs a, i
   using P = typename Frag::P;
   extern __shared__ __align__(16) float ln_sm[];
   __shared__ float red[2 * 2 * R * 32];
+  grid_dependents_go();
   int turn = 0;
   const int groups = blockDim.x / G, gi = threadIdx.x / G, gl = threadIdx.x - gi * G;
   const float rc = 1.f / (float)a.C;
@@ -884,6 +886,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) ln_chan_bwd_k
   using P = typename Word::P;
   constexpr int CPT = chan_cpt<T, W>(), kPairs = Word::kPairs, kChans = Word::kChans, kSlots = CPT / kChans;
   extern __shared__ __align__(16) float ln_sm[];  // [C] (w, w), then [P] x join_warps' pairs
+  grid_dependents_go();
   const int lane = threadIdx.x, s = threadIdx.y, S = blockDim.y, tiles_cta = blockDim.z;
   float2* par = reinterpret_cast<float2*>(ln_sm);
   for (int c = threadIdx.x + 32 * (threadIdx.y + S * threadIdx.z); c < a.C; c += 32 * S * tiles_cta)
@@ -1194,8 +1197,8 @@ int ln_bwd(const LnArgs& a, void* dw, void* db, cudaStream_t s) {
     st = record_launch();
   }
   if (st != MEDNEXT_OK || a.part == nullptr) return st;
-  ln_fold_kernel<<<(a.C + 31) / 32, 1024, 0, s>>>(a.part, parts, a.C, dw, db, a.pdt);
-  return record_launch();
+  return launch_dependent(ln_fold_kernel, dim3((a.C + 31) / 32), dim3(1024), 0, s, (const float*)a.part, parts, a.C, dw,
+                          db, a.pdt);
 }
 
 // Everything that both directions check.  Token and channel counts below 2^31 keep the

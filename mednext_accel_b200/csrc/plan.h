@@ -328,6 +328,24 @@ inline int ensure_smem(K* kern, size_t smem) {
   return smem <= 48 * 1024 ? 0 : ensure_smem_fn(reinterpret_cast<const void*>(kern), smem);
 }
 
+// Launches kern so that it may start before its predecessor in the stream has ended
+// (common.cuh: grid_dependency_wait).  Returns what record_launch() returns.
+template <typename... P, typename... A>
+inline int launch_dependent(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kern, args...);
+  return record_launch();
+}
+
 }  // namespace mednext
 
 // Per-translation-unit reader of the device error word.

@@ -61,17 +61,17 @@ inline bool encode2(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, 
             sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// 8-bit matrix [rows][pitch] of which the first cols columns count (the rest read as
-// zeros), box (128 columns, box_rows), 128-byte swizzle: K-major MMA operands.
-inline bool encode_rows_8bit(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t pitch,
-                             uint32_t box_rows) {
+// 8-bit matrices [mats][rows][pitch] of which the first cols columns count (the rest read
+// as zeros), box (128 columns, box_rows, 1), 128-byte swizzle: K-major MMA operands.
+inline bool encode_rows_8bit(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t mats,
+                             uint64_t pitch, uint32_t box_rows) {
   auto fn = encode_fn();
   if (fn == nullptr) return false;
-  const cuuint64_t dims[2] = {cols, rows};
-  const cuuint64_t strides[1] = {pitch};
-  const cuuint32_t box[2] = {128, box_rows};
-  const cuuint32_t estr[2] = {1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+  const cuuint64_t dims[3] = {cols, rows, mats};
+  const cuuint64_t strides[2] = {pitch, pitch * rows};
+  const cuuint32_t box[3] = {128, box_rows, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
