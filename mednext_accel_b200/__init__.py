@@ -23,6 +23,7 @@ from .grn import (
     install_adaptive_grn,
 )
 from .loss import cross_entropy
+from .mixer import ChannelMixer3d, Int8ChannelMixer3d
 from .network import (
     CheckpointConfig,
     MedNeXtBlock,
@@ -60,10 +61,12 @@ __all__ = [
     "global_response_norm3d_reference",
     "install_adaptive_grn",
     "AdaptivePointwise3d",
+    "ChannelMixer3d",
     "CheckpointConfig",
     "ExecutionContext",
     "ImplementationRegistry",
     "ImplementationSpec",
+    "Int8ChannelMixer3d",
     "Int8Pointwise3d",
     "LayerNorm3d",
     "MedNeXtBlock",

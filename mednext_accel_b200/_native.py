@@ -155,6 +155,7 @@ class CastEntry(ctypes.Structure):
 CAST_MAX_ENTRIES = 16
 
 _lib: ctypes.CDLL | None = None
+_entry: dict[str, object] = {}  # entry points that launch() has looked up
 _device_checked: set[int] = set()
 
 
@@ -229,9 +230,12 @@ def require_device(t: torch.Tensor) -> None:
 def launch(name: str, t: Tensor, *args) -> None:
     """Call entry point ``name`` with ``args`` and the current stream of ``t``'s device,
     that device being current (it need not be the caller's), and check its status."""
+    fn = _entry.get(name)
+    if fn is None:
+        require_device(t)
+        fn = _entry[name] = getattr(load(), name)
     index = t.get_device()
-    fn = getattr(load(), name)
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):

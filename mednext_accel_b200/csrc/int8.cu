@@ -1091,9 +1091,9 @@ int mednext_int8_quantize(const void* x, int8_t* q, float* scale, int64_t outer,
   }
 }
 
-// The workspace holds the tokens' 8-bit rows, then their scales.
+// The workspace holds the tokens' 8-bit rows, then their scales; a few tokens need none.
 size_t mednext_int8_linear_workspace_size(int64_t outer, int64_t k, int64_t inner, int64_t n, int dtype) {
-  if (i8_check(outer, k, inner, dtype) != MEDNEXT_OK || n <= 0) return 0;
+  if (i8_check(outer, k, inner, dtype) != MEDNEXT_OK || n <= 0 || few_takes(outer * inner, (int)k)) return 0;
   const size_t tokens = (size_t)(outer * inner);
   return tokens * (size_t)pitch16(k) + (tokens * sizeof(float) + 15) / 16 * 16;
 }
@@ -1110,9 +1110,8 @@ int mednext_int8_linear(const void* x, const int8_t* weight, const float* weight
   if (x == nullptr || weight == nullptr || weight_scale == nullptr || y == nullptr) return MEDNEXT_ERR_NULL_POINTER;
   if (off(x, elem_size(dtype)) || off(y, elem_size(dtype)) || off(weight, 16) || off(weight_scale, 4) || off(bias, 4))
     return MEDNEXT_ERR_ALIGNMENT;
-  if (workspace == nullptr || off(workspace, 16) ||
-      workspace_bytes < mednext_int8_linear_workspace_size(outer, k, inner, n, dtype))
-    return MEDNEXT_ERR_WORKSPACE;
+  const size_t need = mednext_int8_linear_workspace_size(outer, k, inner, n, dtype);
+  if (need > 0 && (workspace == nullptr || off(workspace, 16) || workspace_bytes < need)) return MEDNEXT_ERR_WORKSPACE;
   int8_t* q = static_cast<int8_t*>(workspace);
   float* qs = reinterpret_cast<float*>(q + (size_t)(outer * inner) * (size_t)pitch16(k));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -126,7 +126,8 @@ def dropout(x: Tensor, p: float, rng: Tensor | tuple[int, int], residual: Tensor
         raise ValueError("dropout requires a probability between 0 and 1")
     state = None
     if isinstance(rng, Tensor):
-        if rng.dtype != torch.int64 or rng.shape != (2,) or rng.device != x.device or not rng.is_contiguous():
+        if (rng.dtype != torch.int64 or rng.ndim != 1 or rng.shape[0] != 2 or rng.get_device() != x.get_device()
+                or not rng.is_contiguous()):
             raise ValueError("dropout requires rng as a contiguous int64 tensor [seed, offset] on the input's device")
         state, seed, offset = rng, layer, 0
     else:
@@ -136,13 +137,15 @@ def dropout(x: Tensor, p: float, rng: Tensor | tuple[int, int], residual: Tensor
     if residual is not None:
         if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
             raise ValueError("dropout requires a residual of the input's shape, type and device")
-        residual = residual.contiguous()
+        if not residual.is_contiguous():
+            residual = residual.contiguous()
     nat.require_device(x)
     drop = round(p * 65536)
-    x = x.contiguous()
+    if not x.is_contiguous():
+        x = x.contiguous()
     seed, offset = _signed(seed), _signed(offset)
     if torch.compiler.is_compiling():
         return dropout_forward(x, residual, state, seed, offset, drop)[0]
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+    if (x.requires_grad or (residual is not None and residual.requires_grad)) and torch.is_grad_enabled():
         return _Dropout.apply(x, residual, state, seed, offset, drop)
     return _launch(x, residual, state, seed, offset, drop, None)

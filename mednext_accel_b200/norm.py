@@ -54,9 +54,11 @@ def in_dense_order(x: Tensor, dim: int) -> tuple[Tensor, int, list[int] | None]:
 
 
 def axis_sizes(x: Tensor, dim: int) -> tuple[int, int, int]:
-    """x.shape as (outer, size of dim, inner)."""
-    shape = x.shape
-    return math.prod(shape[:dim]), shape[dim], math.prod(shape[dim + 1:])
+    """A contiguous x's shape as (outer, size of dim, inner)."""
+    c, inner = x.shape[dim], x.stride(dim)
+    if c < 2 or x.numel() == 0:  # the stride of such an axis may be anything
+        return math.prod(x.shape[:dim]), c, math.prod(x.shape[dim + 1:])
+    return x.numel() // (c * inner), c, inner
 
 
 def _param_code(x: Tensor, weight: Tensor | None, bias: Tensor | None) -> int:
@@ -84,7 +86,7 @@ def _backward(dy: Tensor, x: Tensor, stats: Tensor, weight: Tensor | None, bias:
     ws, nbytes = None, 0
     if dw is not None or db is not None:
         nbytes = nat.load().mednext_ln_bwd_workspace_size(outer, c, inner, code)
-        ws = nat.workspace(nbytes, x.device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     nat.launch("mednext_ln_bwd", x, dy.data_ptr(), x.data_ptr(), stats.data_ptr(), nat.ptr(weight), dx.data_ptr(),
                nat.ptr(dw), nat.ptr(db), nat.ptr(ws), nbytes, outer, c, inner, code, _param_code(x, weight, bias))
     return dx, dw, db
@@ -165,41 +167,48 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
     weight and bias.  The computation runs in x's type, not autocast's."""
     if not x.is_cuda:
         raise ValueError("layer_norm requires CUDA tensors")
-    if x.dtype not in DTYPES:
+    dtype, ndim, index = x.dtype, x.ndim, x.get_device()
+    if dtype not in DTYPES:
         raise ValueError("layer_norm requires a float16, bfloat16 or float32 input")
-    if not -x.ndim <= dim < x.ndim:
-        raise ValueError(f"layer_norm: dim {dim} is out of range for a tensor of {x.ndim} dimensions")
-    dim %= x.ndim
+    if not -ndim <= dim < ndim:
+        raise ValueError(f"layer_norm: dim {dim} is out of range for a tensor of {ndim} dimensions")
+    if dim < 0:
+        dim += ndim
     size = x.shape[dim]
     if size == 0:
         raise ValueError("layer_norm requires a nonempty normalised dimension")
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        if p.device != x.device:
-            raise ValueError(f"layer_norm requires {name} on the input's device")
-        if p.shape != (size,):
-            raise ValueError(f"layer_norm requires {name} with shape ({size},)")
-        if p.dtype != torch.float32 and p.dtype != x.dtype:
-            raise ValueError(f"layer_norm requires a float32 {name}, or one of the input's type")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError("layer_norm requires weight and bias of one type")
-    if not (math.isfinite(eps) and eps > 0):
+    grad = x.requires_grad
+    if weight is not None:
+        weight = _check_param("weight", weight, size, dtype, index)
+        grad = grad or weight.requires_grad
+    if bias is not None:
+        bias = _check_param("bias", bias, size, dtype, index)
+        grad = grad or bias.requires_grad
+        if weight is not None and weight.dtype != bias.dtype:
+            raise ValueError("layer_norm requires weight and bias of one type")
+    if not 0.0 < eps < math.inf:
         raise ValueError("layer_norm requires eps to be finite and positive")
     nat.require_device(x)
-    if weight is not None and not weight.is_contiguous():
-        weight = weight.contiguous()
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
-    x, dim, inverse = in_dense_order(x, dim)
+    inverse = None
+    if not x.is_contiguous():
+        x, dim, inverse = in_dense_order(x, dim)
     if torch.compiler.is_compiling():
         y = layer_norm_forward(x, weight, bias, float(eps), dim)[0]
-    elif torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                      or (bias is not None and bias.requires_grad)):
+    elif grad and torch.is_grad_enabled():
         y = _LayerNorm.apply(x, weight, bias, float(eps), dim)
     else:
         y = _forward(x, weight, bias, float(eps), dim, False)[0]
     return y if inverse is None else y.permute(inverse)
+
+
+def _check_param(name: str, p: Tensor, size: int, dtype: torch.dtype, index: int) -> Tensor:
+    if not p.is_cuda or p.get_device() != index:
+        raise ValueError(f"layer_norm requires {name} on the input's device")
+    if p.ndim != 1 or p.shape[0] != size:
+        raise ValueError(f"layer_norm requires {name} with shape ({size},)")
+    if p.dtype != torch.float32 and p.dtype != dtype:
+        raise ValueError(f"layer_norm requires a float32 {name}, or one of the input's type")
+    return p if p.is_contiguous() else p.contiguous()
 
 
 class LayerNorm3d(nn.Module):

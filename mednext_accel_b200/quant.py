@@ -27,11 +27,12 @@ def _check_input(what: str, x: Tensor, dim: int) -> int:
         raise ValueError(f"{what} requires CUDA tensors")
     if x.dtype not in DTYPES:
         raise ValueError(f"{what} requires a float16, bfloat16 or float32 input")
-    if not -x.ndim <= dim < x.ndim:
-        raise ValueError(f"{what}: dim {dim} is out of range for a tensor of {x.ndim} dimensions")
+    ndim = x.ndim
+    if not -ndim <= dim < ndim:
+        raise ValueError(f"{what}: dim {dim} is out of range for a tensor of {ndim} dimensions")
     if not 0 < x.shape[dim] <= MAX_K:
         raise ValueError(f"{what} requires 1 to {MAX_K} values per token")
-    return dim % x.ndim
+    return dim if dim >= 0 else dim + ndim
 
 
 def quantize_int8(x: Tensor, dim: int = -1) -> tuple[Tensor, Tensor]:
@@ -90,8 +91,8 @@ def int8_linear(x: Tensor, weight: Tensor, scale: Tensor, bias: Tensor | None = 
     them for a float weight's rows (rows whose start is not a multiple of 16 bytes are
     copied on every call); bias: [N] float32 or None."""
     dim = _check_input("int8_linear", x, dim)
-    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)
-                                    or scale.requires_grad):
+    if ((x.requires_grad or scale.requires_grad or (bias is not None and bias.requires_grad))
+            and torch.is_grad_enabled()):
         raise ValueError("int8_linear has no gradient: call it under torch.no_grad(), on detached tensors")
     k = x.shape[dim]
     if weight.dtype != torch.int8 or weight.ndim != 2 or weight.shape[1] != k or weight.shape[0] == 0:
@@ -101,12 +102,17 @@ def int8_linear(x: Tensor, weight: Tensor, scale: Tensor, bias: Tensor | None = 
         raise ValueError(f"int8_linear requires a float32 scale with shape ({n},)")
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,)):
         raise ValueError(f"int8_linear requires a float32 bias with shape ({n},)")
-    if weight.device != x.device or scale.device != x.device or (bias is not None and bias.device != x.device):
+    index = x.get_device()  # -1 for a CPU tensor
+    if weight.get_device() != index or scale.get_device() != index or (bias is not None and bias.get_device() != index):
         raise ValueError("int8_linear requires all tensors on the same CUDA device")
     nat.require_device(x)
-    scale = scale.contiguous()
-    bias = bias.contiguous() if bias is not None else None
-    x, dim, inverse = in_dense_order(x, dim)
+    if not scale.is_contiguous():
+        scale = scale.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    inverse = None
+    if not x.is_contiguous():
+        x, dim, inverse = in_dense_order(x, dim)
     y = int8_linear_op(x, weight, scale, bias, dim) if torch.compiler.is_compiling() else _launch(
         x, weight, scale, bias, dim)
     return y if inverse is None else y.permute(inverse)
