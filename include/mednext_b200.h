@@ -317,7 +317,7 @@ int mednext_ce_bwd(const void* logits, const int64_t* target, const float* fwd_o
  * FLOAT32, BFLOAT16 or FLOAT16; weight / bias [c] in param_dtype (FLOAT32 or dtype),
  * NULL = ones / zeros.  stats: FLOAT32 [outer*inner][2] = (mean, r) for the backward,
  * or NULL.  fp32 arithmetic, one rounding.  No tokens (outer or inner 0) is no work.
- * c <= 2^24, outer*c*inner <= 2^40.  No reference counterpart. */
+ * c <= 2^24 (16384 where inner > 1), outer*c*inner <= 2^40.  No reference counterpart. */
 int mednext_ln_fwd(const void* x, const void* weight, const void* bias, void* y, float* stats,
                    int64_t outer, int64_t c, int64_t inner, float eps, int dtype, int param_dtype,
                    mednext_stream_t stream);

@@ -17,6 +17,7 @@ namespace mednext {
 namespace {
 
 constexpr int kSms = 148;
+constexpr int kChanMost = 16384;  // channels of the channels-first form
 
 struct LnArgs {
   const void* x;
@@ -103,81 +104,6 @@ __global__ void __launch_bounds__(256) ln_rows_any_dx_kernel(LnArgs a) {
   }
 }
 
-// ------------------------------ any width, channels first ------------------------------
-// 32 neighbouring tokens per CTA (lanes), 8 warps over the channels.
-template <typename T>
-__global__ void __launch_bounds__(256) ln_chan_any_fwd_kernel(LnArgs a) {
-  __shared__ float red[8][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long per = (a.inner + 31) / 32, tiles = a.outer * per;
-  for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const long long o = tile / per, v = (tile - o * per) * 32 + lane;
-    const bool in = v < a.inner;
-    const long long base = o * a.C * a.inner + v;
-    const T* x = static_cast<const T*>(a.x) + base;
-    T* y = static_cast<T*>(a.y) + base;
-    float stat[2];
-    for (int pass = 0; pass < 2; ++pass) {
-      float s = 0.f;
-      for (int c = warp; c < a.C; c += 8) {
-        const float d = in ? to_acc<T>(x[(long long)c * a.inner]) - (pass ? stat[0] : 0.f) : 0.f;
-        s += pass ? d * d : d;
-      }
-      __syncthreads();
-      red[warp][lane] = s;
-      __syncthreads();
-      s = 0.f;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) s += red[w][lane];
-      stat[pass] = pass ? rsqrtf(s / (float)a.C + a.eps) : s / (float)a.C;
-    }
-    if (!in) continue;
-    for (int c = warp; c < a.C; c += 8)
-      y[(long long)c * a.inner] = from_acc<T>(fmaf((to_acc<T>(x[(long long)c * a.inner]) - stat[0]) * stat[1],
-                                                   load_param(a.w, a.pdt, c, 1.f), load_param(a.b, a.pdt, c, 0.f)));
-    if (a.stats != nullptr && warp == 0) a.stats[o * a.inner + v] = make_float2(stat[0], stat[1]);
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) ln_chan_any_dx_kernel(LnArgs a) {
-  __shared__ float2 red[8][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long per = (a.inner + 31) / 32, tiles = a.outer * per;
-  for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const long long o = tile / per, v = (tile - o * per) * 32 + lane;
-    const bool in = v < a.inner;
-    const long long base = o * a.C * a.inner + v;
-    const T* x = static_cast<const T*>(a.x) + base;
-    const T* dy = static_cast<const T*>(a.dy) + base;
-    T* dx = static_cast<T*>(a.y) + base;
-    const float2 st = in ? a.stats[o * a.inner + v] : make_float2(0.f, 0.f);
-    float2 s = make_float2(0.f, 0.f);
-    if (in)
-      for (int c = warp; c < a.C; c += 8) {
-        const float g = to_acc<T>(dy[(long long)c * a.inner]) * load_param(a.w, a.pdt, c, 1.f);
-        s.x += g;
-        s.y = fmaf(g, (to_acc<T>(x[(long long)c * a.inner]) - st.x) * st.y, s.y);
-      }
-    __syncthreads();
-    red[warp][lane] = s;
-    __syncthreads();
-    s = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      s.x += red[w][lane].x;
-      s.y += red[w][lane].y;
-    }
-    const float m1 = s.x / (float)a.C, m2 = s.y / (float)a.C;
-    if (in)
-      for (int c = warp; c < a.C; c += 8) {
-        const float g = to_acc<T>(dy[(long long)c * a.inner]) * load_param(a.w, a.pdt, c, 1.f);
-        dx[(long long)c * a.inner] =
-            from_acc<T>(st.y * (g - m1 - (to_acc<T>(x[(long long)c * a.inner]) - st.x) * st.y * m2));
-      }
-  }
-}
-
 // ------------------------------ weight-grad partials, any width ------------------------------
 // Rows: a CTA owns 32 columns x one part of the tokens, 8 warps striding its rows.
 template <typename T>
@@ -202,28 +128,6 @@ __global__ void __launch_bounds__(256) ln_rows_any_dw_kernel(LnArgs a, int parts
       s.x += red[w][lane].x;
       s.y += red[w][lane].y;
     }
-    a.part[((long long)p * 2) * a.C + c] = s.x;
-    a.part[((long long)p * 2 + 1) * a.C + c] = s.y;
-  }
-}
-
-// Channels first: a CTA owns one channel x one part of the tokens.
-template <typename T>
-__global__ void __launch_bounds__(256) ln_chan_any_dw_kernel(LnArgs a, int parts) {
-  __shared__ float2 red[32];
-  const int c = blockIdx.x, p = blockIdx.y;
-  const long long per = (a.tokens + parts - 1) / parts;
-  const long long t0 = p * per, t1 = min(t0 + per, a.tokens);
-  float2 s = make_float2(0.f, 0.f);
-  for (long long t = t0 + threadIdx.x; t < t1; t += blockDim.x) {
-    const long long o = t / a.inner, v = t - o * a.inner, i = (o * a.C + c) * a.inner + v;
-    const float2 st = a.stats[t];
-    const float d = to_acc<T>(static_cast<const T*>(a.dy)[i]);
-    s.x = fmaf(d, (to_acc<T>(static_cast<const T*>(a.x)[i]) - st.x) * st.y, s.x);
-    s.y += d;
-  }
-  s = cta_sum2(s.x, s.y, red);
-  if (threadIdx.x == 0) {
     a.part[((long long)p * 2) * a.C + c] = s.x;
     a.part[((long long)p * 2 + 1) * a.C + c] = s.y;
   }
@@ -763,57 +667,99 @@ __device__ __forceinline__ void fold_slot(float2* p) {
   if (W == 1) p[0] = f2(p[0].x + p[0].y);
 }
 
-template <typename T, int W, int THREADS>
+// LOOP: more channels than S warps hold at once: a warp goes through its share CPT at a time,
+// once for the statistics and once more (from L2) for y.
+template <typename T, int W, int THREADS, bool LOOP>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) ln_chan_fwd_kernel(LnArgs a) {
   using Word = TokenWord<T, W>;
   using P = typename Word::P;
   constexpr int CPT = chan_cpt<T, W>(), kPairs = Word::kPairs, kChans = Word::kChans, kSlots = CPT / kChans;
-  extern __shared__ __align__(16) float ln_sm[];  // [C] (w, w, b, b), then [P] x join_warps' pairs
+  extern __shared__ __align__(16) float ln_sm[];  // [C] (w, w, b, b) unless LOOP, then [P] x join_warps' pairs
   const int lane = threadIdx.x, s = threadIdx.y, S = blockDim.y, tiles_cta = blockDim.z;
   float4* par = reinterpret_cast<float4*>(ln_sm);
-  for (int c = threadIdx.x + 32 * (threadIdx.y + S * threadIdx.z); c < a.C; c += 32 * S * tiles_cta) {
-    const float w = load_param(a.w, a.pdt, c, 1.f), b = load_param(a.b, a.pdt, c, 0.f);
-    par[c] = make_float4(w, w, b, b);
+  if (!LOOP) {
+    for (int c = threadIdx.x + 32 * (threadIdx.y + S * threadIdx.z); c < a.C; c += 32 * S * tiles_cta) {
+      const float w = load_param(a.w, a.pdt, c, 1.f), b = load_param(a.b, a.pdt, c, 0.f);
+      par[c] = make_float4(w, w, b, b);
+    }
   }
-  float2* red = reinterpret_cast<float2*>(par + a.C) + threadIdx.z * (S + 1) * W * 32;
+  float2* red = reinterpret_cast<float2*>(par + (LOOP ? 0 : a.C)) + threadIdx.z * (S + 1) * W * 32;
   __syncthreads();
   const long long per = (a.inner + 32 * W - 1) / (32 * W), tiles = a.outer * per;
   const float rc = 1.f / (float)a.C;
   const int share = a.C / S, more = a.C - share * S;  // warp i has share channels, one more where i < more
-  const int mine = share + (s < more ? 1 : 0);
-  const float rmine = 1.f / (float)mine;
+  const int all = share + (s < more ? 1 : 0);
+  // (w, w, b, b) of this warp's slot from channel k on; W = 1: of two channels
+  const auto params = [&](int k, bool two) {
+    const int c = k * S + s;
+    float4 wb;
+    if (LOOP) {
+      wb = make_float4(load_param(a.w, a.pdt, c, 1.f), 0.f, load_param(a.b, a.pdt, c, 0.f), 0.f);
+      wb.y = two ? load_param(a.w, a.pdt, c + S, 1.f) : wb.x;
+      wb.w = two ? load_param(a.b, a.pdt, c + S, 0.f) : wb.z;
+    } else {
+      wb = lds4(par + c);
+      if (two) {
+        const float4 next = lds4(par + c + S);
+        wb.y = next.y;
+        wb.w = next.w;
+      }
+    }
+    return wb;
+  };
   for (long long base = (long long)blockIdx.x * tiles_cta; base < tiles; base += (long long)gridDim.x * tiles_cta) {
     const long long tile = base + threadIdx.z;
     const long long o = tile / per, v = (tile - o * per) * (32 * W) + lane * W;
     const bool in = tile < tiles && v < a.inner;  // inner is a multiple of W
     const long long at = (o * a.C + s) * a.inner + v, step = (long long)S * a.inner;
     Word x[kSlots];
-    const T* px = static_cast<const T*>(a.x) + at;
+    const auto load = [&](int first) {  // this warp's channels from `first` on
+      const T* px = static_cast<const T*>(a.x) + at + first * step;
 #pragma unroll
-    for (int k = 0; k < kSlots; ++k, advance(px, step * kChans)) x[k].load(px, in ? mine - k * kChans : 0, step);
-    // this warp's mean and squares about it; the warps' join below (Chan, Golub and LeVeque)
+      for (int k = 0; k < kSlots; ++k, advance(px, step * kChans)) x[k].load(px, in ? all - first - k * kChans : 0, step);
+    };
+    // this warp's mean and squares about it; the pieces and the warps' join (Chan, Golub and LeVeque)
     float2 nm[kPairs], m2[kPairs];
 #pragma unroll
     for (int j = 0; j < kPairs; ++j) nm[j] = m2[j] = make_float2(0.f, 0.f);
+    for (int first = 0; first < (LOOP ? all : 1); first += CPT) {
+      const int mine = LOOP ? min(CPT, all - first) : all;
+      load(first);
+      float2 pm[kPairs], p2[kPairs];
 #pragma unroll
-    for (int k = 0; k < kSlots; ++k)
+      for (int j = 0; j < kPairs; ++j) pm[j] = p2[j] = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int j = 0; j < kPairs; ++j) nm[j] = P::plus(x[k].w[j], nm[j]);
-    fold_slot<W>(nm);
+      for (int k = 0; k < kSlots; ++k)
 #pragma unroll
-    for (int j = 0; j < kPairs; ++j) nm[j] = __fmul2_rn(nm[j], f2(-rmine));
+        for (int j = 0; j < kPairs; ++j) pm[j] = P::plus(x[k].w[j], pm[j]);
+      fold_slot<W>(pm);
 #pragma unroll
-    for (int k = 0; k < kSlots; ++k)
-      if (k * kChans < mine) {
-        x[k].again();
+      for (int j = 0; j < kPairs; ++j) pm[j] = __fmul2_rn(pm[j], f2(-1.f / (float)mine));
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          float2 d = P::plus(x[k].w[j], nm[j]);
-          if (W == 1 && k * kChans + 1 >= mine) d.y = 0.f;
-          m2[j] = __ffma2_rn(d, d, m2[j]);
+      for (int k = 0; k < kSlots; ++k)
+        if (k * kChans < mine) {
+          x[k].again();
+#pragma unroll
+          for (int j = 0; j < kPairs; ++j) {
+            float2 d = P::plus(x[k].w[j], pm[j]);
+            if (W == 1 && k * kChans + 1 >= mine) d.y = 0.f;
+            p2[j] = __ffma2_rn(d, d, p2[j]);
+          }
+        }
+      fold_slot<W>(p2);
+      const float na = (float)first, nb = (float)mine, share_b = nb / (na + nb);
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) {
+        if (!LOOP) {
+          nm[j] = pm[j];
+          m2[j] = p2[j];
+        } else {
+          const float2 d = __fadd2_rn(pm[j], make_float2(-nm[j].x, -nm[j].y));
+          nm[j] = __ffma2_rn(d, f2(share_b), nm[j]);
+          m2[j] = __fadd2_rn(m2[j], __ffma2_rn(__fmul2_rn(d, d), f2(na * share_b), p2[j]));
         }
       }
-    fold_slot<W>(m2);
+    }
     float2 rstd[kPairs];
     float2 st[W];
 #pragma unroll
@@ -837,24 +783,23 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) ln_chan_fwd_k
       set_token<W>(rstd, j, st[j].y);
     }
     if (in) {
-      T* y = static_cast<T*>(a.y) + at;
+      for (int first = 0; first < (LOOP ? all : 1); first += CPT) {
+        const int mine = LOOP ? min(CPT, all - first) : all;
+        if (LOOP) load(first);
+        T* y = static_cast<T*>(a.y) + at + first * step;
 #pragma unroll
-      for (int k = 0; k < kSlots; ++k, advance(y, step * kChans))
-        if (k * kChans < mine) {
-          float4 wb = lds4(par + k * kChans * S + s);
-          if (W == 1 && k * kChans + 1 < mine) {
-            const float4 next = lds4(par + (k * kChans + 1) * S + s);
-            wb.y = next.y;
-            wb.w = next.w;
+        for (int k = 0; k < kSlots; ++k, advance(y, step * kChans))
+          if (k * kChans < mine) {
+            const float4 wb = params(first + k * kChans, W == 1 && k * kChans + 1 < mine);
+            float2 f[kPairs];
+            x[k].again();
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j)
+              f[j] = __ffma2_rn(__fmul2_rn(P::plus(x[k].w[j], nm[j]), rstd[j]), make_float2(wb.x, wb.y),
+                                make_float2(wb.z, wb.w));
+            Word::store(y, mine - k * kChans, step, f);
           }
-          float2 f[kPairs];
-          x[k].again();
-#pragma unroll
-          for (int j = 0; j < kPairs; ++j)
-            f[j] = __ffma2_rn(__fmul2_rn(P::plus(x[k].w[j], nm[j]), rstd[j]), make_float2(wb.x, wb.y),
-                              make_float2(wb.z, wb.w));
-          Word::store(y, mine - k * kChans, step, f);
-        }
+      }
       if (a.stats != nullptr && s == 0) {
 #pragma unroll
         for (int j = 0; j < W; ++j) a.stats[o * a.inner + v + j] = make_float2(-st[j].x, st[j].y);
@@ -880,25 +825,30 @@ __device__ __forceinline__ float transpose_sum(float (&v)[N], int lane) {
   return v[0];
 }
 
-template <typename T, int W, int THREADS>
+// LOOP: as forward; x and dy are read twice, and a channel's weight-grad sums are kept in
+// shared memory by the lane that owns it.
+template <typename T, int W, int THREADS, bool LOOP>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) ln_chan_bwd_kernel(LnArgs a) {
   using Word = TokenWord<T, W>;
   using P = typename Word::P;
   constexpr int CPT = chan_cpt<T, W>(), kPairs = Word::kPairs, kChans = Word::kChans, kSlots = CPT / kChans;
-  extern __shared__ __align__(16) float ln_sm[];  // [C] (w, w), then [P] x join_warps' pairs
+  // [C] (w, w), or (dw, db) where LOOP; then [P] x join_warps' pairs
+  extern __shared__ __align__(16) float ln_sm[];
   grid_dependents_go();
   const int lane = threadIdx.x, s = threadIdx.y, S = blockDim.y, tiles_cta = blockDim.z;
   float2* par = reinterpret_cast<float2*>(ln_sm);
   for (int c = threadIdx.x + 32 * (threadIdx.y + S * threadIdx.z); c < a.C; c += 32 * S * tiles_cta)
-    par[c] = f2(load_param(a.w, a.pdt, c, 1.f));
+    par[c] = LOOP ? make_float2(0.f, 0.f) : f2(load_param(a.w, a.pdt, c, 1.f));
   float2* red = par + a.C + threadIdx.z * (S + 1) * W * 32;
   __syncthreads();
   const long long per = (a.inner + 32 * W - 1) / (32 * W), tiles = a.outer * per;
   const float rc = 1.f / (float)a.C;
-  const int mine = a.C / S + (s < a.C % S ? 1 : 0);
-  const auto weight = [=](int k) {  // of slot k
-    float2 w = lds2(par + k * kChans * S + s);
-    if (W == 1 && k * kChans + 1 < mine) w.y = lds2(par + (k * kChans + 1) * S + s).y;
+  const int all = a.C / S + (s < a.C % S ? 1 : 0);
+  const auto weight = [&](int k, bool two) {  // of this warp's slot from channel k on
+    const int c = k * S + s;
+    if (LOOP) return make_float2(load_param(a.w, a.pdt, c, 1.f), load_param(a.w, a.pdt, two ? c + S : c, 1.f));
+    float2 w = lds2(par + c);
+    if (two) w.y = lds2(par + c + S).y;
     return w;
   };
   float dw = 0.f, db = 0.f;  // of channel (lane % CPT) * S + s
@@ -908,12 +858,15 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) ln_chan_bwd_k
     const bool in = tile < tiles && v < a.inner;
     const long long at = (o * a.C + s) * a.inner + v, step = (long long)S * a.inner;
     Word x[kSlots], d[kSlots];
-    const T *px = static_cast<const T*>(a.x) + at, *pd = static_cast<const T*>(a.dy) + at;
+    const auto load = [&](int first) {
+      const T *px = static_cast<const T*>(a.x) + at + first * step, *pd = static_cast<const T*>(a.dy) + at + first * step;
 #pragma unroll
-    for (int k = 0; k < kSlots; ++k, advance(px, step * kChans), advance(pd, step * kChans)) {
-      x[k].load(px, in ? mine - k * kChans : 0, step);
-      d[k].load(pd, in ? mine - k * kChans : 0, step);
-    }
+      for (int k = 0; k < kSlots; ++k, advance(px, step * kChans), advance(pd, step * kChans)) {
+        x[k].load(px, in ? all - first - k * kChans : 0, step);
+        d[k].load(pd, in ? all - first - k * kChans : 0, step);
+      }
+    };
+    if (!LOOP) load(0);
     float2 nm[kPairs], r[kPairs], s1[kPairs], s2[kPairs];
 #pragma unroll
     for (int j = 0; j < W; ++j) {
@@ -923,19 +876,23 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) ln_chan_bwd_k
     }
 #pragma unroll
     for (int j = 0; j < kPairs; ++j) s1[j] = s2[j] = make_float2(0.f, 0.f);
+    for (int first = 0; first < (LOOP ? all : 1); first += CPT) {
+      const int mine = LOOP ? min(CPT, all - first) : all;
+      if (LOOP) load(first);
 #pragma unroll
-    for (int k = 0; k < kSlots; ++k)
-      if (k * kChans < mine) {
-        const float2 w = weight(k);
+      for (int k = 0; k < kSlots; ++k)
+        if (k * kChans < mine) {
+          const float2 w = weight(first + k * kChans, W == 1 && k * kChans + 1 < mine);
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          // sum of g (x - mean): the common r is multiplied once, below.  An absent second
-          // channel (W = 1) has dy = 0.
-          const float2 gw = __fmul2_rn(P::value(d[k].w[j]), w);
-          s1[j] = __fadd2_rn(s1[j], gw);
-          s2[j] = __ffma2_rn(gw, P::plus(x[k].w[j], nm[j]), s2[j]);
+          for (int j = 0; j < kPairs; ++j) {
+            // sum of g (x - mean): the common r is multiplied once, below.  An absent second
+            // channel (W = 1) has dy = 0.
+            const float2 gw = __fmul2_rn(P::value(d[k].w[j]), w);
+            s1[j] = __fadd2_rn(s1[j], gw);
+            s2[j] = __ffma2_rn(gw, P::plus(x[k].w[j], nm[j]), s2[j]);
+          }
         }
-      }
+    }
     fold_slot<W>(s1);
     fold_slot<W>(s2);
     if (S > 1) {
@@ -958,57 +915,74 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) ln_chan_bwd_k
       s1[j] = __fmul2_rn(s1[j], f2(-rc));                    // -mean(g)
       s2[j] = __fmul2_rn(__fmul2_rn(s2[j], r[j]), f2(-rc));  // -mean(g xh)
     }
-    float pw[CPT], pb[CPT];
-    T* dx = static_cast<T*>(a.y) + at;
+    for (int first = 0; first < (LOOP ? all : 1); first += CPT) {
+      const int mine = LOOP ? min(CPT, all - first) : all;
+      if (LOOP) load(first);
+      float pw[CPT], pb[CPT];
+      T* dx = static_cast<T*>(a.y) + at + first * step;
 #pragma unroll
-    for (int k = 0; k < kSlots; ++k, advance(dx, step * kChans)) {
-      float2 tw = make_float2(0.f, 0.f), tb = tw;
-      if (k * kChans < mine) {
-        const float2 w = weight(k);
-        float2 f[kPairs];
-        x[k].again();
-        d[k].again();
+      for (int k = 0; k < kSlots; ++k, advance(dx, step * kChans)) {
+        float2 tw = make_float2(0.f, 0.f), tb = tw;
+        if (k * kChans < mine) {
+          const float2 w = weight(first + k * kChans, W == 1 && k * kChans + 1 < mine);
+          float2 f[kPairs];
+          x[k].again();
+          d[k].again();
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          const float2 g = P::value(d[k].w[j]), xh = __fmul2_rn(P::plus(x[k].w[j], nm[j]), r[j]);
-          tw = __ffma2_rn(g, xh, tw);
-          tb = __fadd2_rn(tb, g);
-          f[j] = __fmul2_rn(__ffma2_rn(xh, s2[j], __ffma2_rn(g, w, s1[j])), r[j]);
+          for (int j = 0; j < kPairs; ++j) {
+            const float2 g = P::value(d[k].w[j]), xh = __fmul2_rn(P::plus(x[k].w[j], nm[j]), r[j]);
+            tw = __ffma2_rn(g, xh, tw);
+            tb = __fadd2_rn(tb, g);
+            f[j] = __fmul2_rn(__ffma2_rn(xh, s2[j], __ffma2_rn(g, w, s1[j])), r[j]);
+          }
+          if (in) Word::store(dx, mine - k * kChans, step, f);
         }
-        if (in) Word::store(dx, mine - k * kChans, step, f);
+        if constexpr (W == 1) {
+          pw[2 * k] = tw.x;
+          pw[2 * k + 1] = tw.y;
+          pb[2 * k] = tb.x;
+          pb[2 * k + 1] = tb.y;
+        } else {
+          pw[k] = tw.x + tw.y;
+          pb[k] = tb.x + tb.y;
+        }
       }
-      if constexpr (W == 1) {
-        pw[2 * k] = tw.x;
-        pw[2 * k + 1] = tw.y;
-        pb[2 * k] = tb.x;
-        pb[2 * k + 1] = tb.y;
-      } else {
-        pw[k] = tw.x + tw.y;
-        pb[k] = tb.x + tb.y;
+      if (a.part != nullptr) {
+        const float2 t = make_float2(transpose_sum<CPT>(pw, lane), transpose_sum<CPT>(pb, lane));
+        if (!LOOP) {
+          dw += t.x;
+          db += t.y;
+        } else if (lane < mine) {  // LOOP has one tile per CTA at a time: this warp's alone
+          float2* acc = par + (first + lane) * S + s;
+          *acc = __fadd2_rn(*acc, t);
+        }
       }
-    }
-    if (a.part != nullptr) {
-      dw += transpose_sum<CPT>(pw, lane);
-      db += transpose_sum<CPT>(pb, lane);
     }
   }
   if (a.part == nullptr) return;
   // the CTA's tiles, in order, then one partial per CTA
   __syncthreads();
+  float* part = a.part + (long long)blockIdx.x * 2 * a.C;
+  if (LOOP) {
+    for (int c = threadIdx.x + 32 * threadIdx.y; c < a.C; c += 32 * S) {
+      part[c] = par[c].x;
+      part[a.C + c] = par[c].y;
+    }
+    return;
+  }
   float2* acc = par + a.C;  // [P][S][32]
   acc[(threadIdx.z * S + s) * 32 + lane] = make_float2(dw, db);
   __syncthreads();
-  if (threadIdx.z == 0 && lane < mine) {
+  if (threadIdx.z == 0 && lane < all) {
     float2 t = acc[s * 32 + lane];
     for (int p = 1; p < tiles_cta; ++p) t = __fadd2_rn(t, acc[(p * S + s) * 32 + lane]);
-    float* part = a.part + (long long)blockIdx.x * 2 * a.C;
     part[lane * S + s] = t.x;
     part[a.C + lane * S + s] = t.y;
   }
 }
 
 // ------------------------------ host side ------------------------------
-// How a call runs.  kAny covers what does not fit into registers.
+// How a call runs.  kAny: rows that do not fit into registers.
 enum LnForm { kRows, kChan, kAny };
 struct LnPlan {
   LnForm form;
@@ -1017,6 +991,7 @@ struct LnPlan {
   int G;            // kRows: threads per row
   int threads;      // kRows: of a CTA
   int S, P;         // kChan: warps per tile, tiles per CTA
+  bool loop;        // kChan: more channels than the warps hold
   long long units;  // CTA-sized pieces of work
 };
 
@@ -1041,22 +1016,30 @@ LnPlan plan_rows(long long tokens, int C, int vec) {
 }
 
 // Channels first: the widest word that the alignment allows and whose tile has enough
-// warps for C: 32 forward, 16 backward (its threads hold x and dy).
+// warps for C: 32 forward, 16 backward (its threads hold x and dy); more channels than any
+// holds are gone through in a loop, with the widest word.  Backward, LOOP keeps 8 bytes per
+// channel in shared memory: up to 16384 of them.
 LnPlan plan_chan(long long outer, long long inner, int C, size_t esz, size_t align, bool bwd) {
   LnPlan p{};
-  p.form = kAny;
   const int most = bwd ? 16 : 32;
+  p.form = kChan;
+  int widest = 1;
   for (int w = (int)(8 / esz); w >= 1; w /= 2) {
     if (inner % w != 0 || align % (w * esz) != 0) continue;
+    widest = std::max(widest, w);
     const int cpt = w * (int)esz == 8 ? 16 : 32;
     p.S = (C + cpt - 1) / cpt;
     if (p.S > most) continue;
-    p.form = kChan;
     p.vec = w;
     p.P = std::max(1, 4 / p.S);
     p.units = (outer * ((inner + 32 * w - 1) / (32 * w)) + p.P - 1) / p.P;
     return p;
   }
+  p.loop = true;
+  p.vec = widest;
+  p.S = most;
+  p.P = 1;
+  p.units = outer * ((inner + 32 * widest - 1) / (32 * widest));
   return p;
 }
 
@@ -1121,19 +1104,19 @@ int launch_rows_any_vec(const LnArgs& a, const LnPlan& p, bool bwd, int parts, c
   return launch_rows_vec<T, 16 / sizeof(T)>(a, p, bwd, parts, s);
 }
 
-template <typename T, int W, int FWD_THREADS, int BWD_THREADS>
+template <typename T, int W, int FWD_THREADS, int BWD_THREADS, bool LOOP>
 int launch_chan(const LnArgs& a, const LnPlan& p, bool bwd, int parts, cudaStream_t s) {
   const size_t red = (size_t)p.P * (p.S + 1) * W * 32 * sizeof(float2);
   const dim3 block(32, p.S, p.P);
   if (!bwd) {
-    auto kern = ln_chan_fwd_kernel<T, W, FWD_THREADS>;
-    const size_t smem = (size_t)a.C * sizeof(float4) + red;
+    auto kern = ln_chan_fwd_kernel<T, W, FWD_THREADS, LOOP>;
+    const size_t smem = (LOOP ? 0 : (size_t)a.C * sizeof(float4)) + red;
     const int st = ensure_smem(kern, smem);
     if (st != MEDNEXT_OK) return st;
     const long long cap = kSms * (long long)std::max(1, 24 / (p.S * p.P));  // resident: 24 warps
     kern<<<(unsigned)std::min(p.units, cap), block, smem, s>>>(a);
   } else {
-    auto kern = ln_chan_bwd_kernel<T, W, BWD_THREADS>;
+    auto kern = ln_chan_bwd_kernel<T, W, BWD_THREADS, LOOP>;
     const size_t smem = (size_t)a.C * sizeof(float2) + red;
     const int st = ensure_smem(kern, smem);
     if (st != MEDNEXT_OK) return st;
@@ -1143,7 +1126,9 @@ int launch_chan(const LnArgs& a, const LnPlan& p, bool bwd, int parts, cudaStrea
 }
 template <typename T, int W>
 int launch_chan_word(const LnArgs& a, const LnPlan& p, bool bwd, int parts, cudaStream_t s) {
-  return p.S <= 8 ? launch_chan<T, W, 256, 256>(a, p, bwd, parts, s) : launch_chan<T, W, 1024, 512>(a, p, bwd, parts, s);
+  if (p.loop) return launch_chan<T, W, 1024, 512, true>(a, p, bwd, parts, s);
+  return p.S <= 8 ? launch_chan<T, W, 256, 256, false>(a, p, bwd, parts, s)
+                  : launch_chan<T, W, 1024, 512, false>(a, p, bwd, parts, s);
 }
 template <typename T>
 int launch_chan_any_word(const LnArgs& a, const LnPlan& p, bool bwd, int parts, cudaStream_t s) {
@@ -1158,12 +1143,7 @@ int ln_fwd(const LnArgs& a, cudaStream_t s) {
   const LnPlan p = plan_ln<T>(a, false);
   if (p.form == kRows) return launch_rows_any_vec<T>(a, p, false, 0, s);
   if (p.form == kChan) return launch_chan_any_word<T>(a, p, false, 0, s);
-  if (a.inner == 1) {
-    ln_rows_any_fwd_kernel<T><<<(unsigned)std::min<long long>(a.tokens, kSms * 32), 256, 0, s>>>(a);
-  } else {
-    const long long tiles = a.outer * ((a.inner + 31) / 32);
-    ln_chan_any_fwd_kernel<T><<<(unsigned)std::min<long long>(tiles, kSms * 32), 256, 0, s>>>(a);
-  }
+  ln_rows_any_fwd_kernel<T><<<(unsigned)std::min<long long>(a.tokens, kSms * 32), 256, 0, s>>>(a);
   return record_launch();
 }
 
@@ -1180,20 +1160,12 @@ int ln_bwd(const LnArgs& a, void* dw, void* db, cudaStream_t s) {
     st = launch_chan_any_word<T>(a, p, true, parts, s);
   } else {
     // enough CTAs for the GPU over the columns and the parts
-    const long long cols = a.inner == 1 ? (a.C + 31) / 32 : a.C;
+    const long long cols = (a.C + 31) / 32;
     parts = (int)std::min<long long>(dw_parts(a.tokens), std::max(1LL, (long long)kSms * 8 / cols));
-    if (a.inner == 1) {
-      ln_rows_any_dx_kernel<T><<<(unsigned)std::min<long long>(a.tokens, kSms * 32), 256, 0, s>>>(a);
-    } else {
-      const long long tiles = a.outer * ((a.inner + 31) / 32);
-      ln_chan_any_dx_kernel<T><<<(unsigned)std::min<long long>(tiles, kSms * 32), 256, 0, s>>>(a);
-    }
+    ln_rows_any_dx_kernel<T><<<(unsigned)std::min<long long>(a.tokens, kSms * 32), 256, 0, s>>>(a);
     st = record_launch();
     if (st != MEDNEXT_OK || a.part == nullptr) return st;
-    if (a.inner == 1)
-      ln_rows_any_dw_kernel<T><<<dim3((a.C + 31) / 32, parts), 256, 0, s>>>(a, parts);
-    else
-      ln_chan_any_dw_kernel<T><<<dim3(a.C, parts), 256, 0, s>>>(a, parts);
+    ln_rows_any_dw_kernel<T><<<dim3((unsigned)cols, parts), 256, 0, s>>>(a, parts);
     st = record_launch();
   }
   if (st != MEDNEXT_OK || a.part == nullptr) return st;
@@ -1207,6 +1179,7 @@ int ln_check(int64_t outer, int64_t c, int64_t inner, int dtype, int param_dtype
   if (dtype != MEDNEXT_FLOAT32 && dtype != MEDNEXT_BFLOAT16 && dtype != MEDNEXT_FLOAT16) return MEDNEXT_ERR_BAD_DTYPE;
   if (param_dtype != MEDNEXT_FLOAT32 && param_dtype != dtype) return MEDNEXT_ERR_BAD_DTYPE;
   if (outer < 0 || inner < 0 || c <= 0 || c > ((int64_t)1 << 24)) return MEDNEXT_ERR_BAD_SHAPE;
+  if (inner > 1 && c > kChanMost) return MEDNEXT_ERR_BAD_SHAPE;
   const int64_t lim = (int64_t)1 << 40;  // tokens, and elements
   if (outer >= lim || inner >= lim) return MEDNEXT_ERR_BAD_SHAPE;
   if (outer > 0 && inner > 0 && (inner > lim / outer || outer * inner > lim / c)) return MEDNEXT_ERR_BAD_SHAPE;

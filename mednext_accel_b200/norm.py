@@ -29,6 +29,7 @@ from torch.library import custom_op
 from . import _native as nat
 
 _NS = "mednext_accel_b200"
+CHANNELS_MOST = 16384  # of the channels-first kernels
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
@@ -192,6 +193,9 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
     inverse = None
     if not x.is_contiguous():
         x, dim, inverse = in_dense_order(x, dim)
+    if size > CHANNELS_MOST and x.stride(dim) > 1:  # past the channels-first kernels: as rows, by copies
+        y = layer_norm(x.movedim(dim, -1).contiguous(), weight, bias, eps).movedim(-1, dim).contiguous()
+        return y if inverse is None else y.permute(inverse)
     if torch.compiler.is_compiling():
         y = layer_norm_forward(x, weight, bias, float(eps), dim)[0]
     elif grad and torch.is_grad_enabled():

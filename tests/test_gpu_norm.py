@@ -322,3 +322,15 @@ def test_refusals():
     ):
         with pytest.raises(ValueError, match=text):
             mx.layer_norm(*args, **kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 600, 2048), (2, 1000, 777), (1, 1025, 256), (1, 4096, 40), (1, 16384, 9), (1, 16385, 3)])
+def test_channels_first_wide(shape, dtype):
+    """More channels than a tile's warps hold at once, and than the channels-first form has."""
+    x, w, b, dy = inputs(shape, 1, dtype, seed=sum(shape))
+    check(x, w, b, dy, 1)
+    if shape[1] > 16384:
+        check(x.transpose(1, 2).contiguous().transpose(1, 2), w, b, dy, 1)
+        y = x.permute(1, 2, 0).contiguous().permute(2, 0, 1)
+        check(y, w, b, dy, 1)
