@@ -219,13 +219,26 @@ __device__ __forceinline__ void renew(uint32_t& v) { asm volatile("" : "+r"(v));
 __device__ __forceinline__ void renew(float2&) {}
 __device__ __forceinline__ void renew(Halves& v) { asm volatile("" : "+h"(v.a), "+h"(v.b)); }
 
+// A 16-byte load that is issued where it is written (zeros if not ok): left to itself the
+// compiler sinks the loads for the next rows behind the work on these.
+__device__ __forceinline__ uint4 load_here(const void* p, bool ok) {
+  uint4 q;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %5, 0;\n\t"
+      "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+      "@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(q.x), "=&r"(q.y), "=&r"(q.z), "=&r"(q.w)
+      : "l"(p), "r"((uint32_t)ok));
+  return q;
+}
+
 // ------------------------------ rows held in registers ------------------------------
 // G threads hold a row, EPT elements each, in words of VEC elements (16 bytes; 4 bytes or
 // single elements where rows do not start on 16), word v of thread gl beginning at column
 // (v G + gl) VEC.  G <= 32 is a power of two and its sums are shuffles; wider rows take
-// whole warps, which add through shared memory, one barrier per sum, R rows at once.
-// Up to 1024 columns are one warp's: 32 elements per thread cost 10 shuffles for two
-// sums, against two barriers per row for more warps with fewer elements.
+// whole warps, which add through shared memory, one barrier of the group per sum, R rows at
+// once.
 template <typename T, int VEC, int EPT>
 struct RowFrag {
   using P = PackFor<T, VEC == 1>;
@@ -247,7 +260,7 @@ struct RowFrag {
         const int c = col(j, 0, gl, G);
         const bool ok = in && c < C;
         if constexpr (sizeof(T) * VEC == 16) {
-          const uint4 q = ok ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+          const uint4 q = load_here(row + c, ok);
           if constexpr (sizeof(T) == 4) {
             w[2 * j] = make_float2(__uint_as_float(q.x), __uint_as_float(q.y));
             w[2 * j + 1] = make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
@@ -357,7 +370,8 @@ __device__ __forceinline__ void group_sum(float (&v)[N], int G, float* red, int&
 #pragma unroll
     for (int n = 0; n < N; ++n) r[n * 32 + warp] = v[n];
   }
-  __syncthreads();
+  // the groups of a CTA go their own ways
+  asm volatile("bar.sync %0, %1;" ::"r"((int)threadIdx.x / G + 1), "r"(G) : "memory");
   const int w0 = (threadIdx.x / G) * (G >> 5), w1 = w0 + (G >> 5);
 #pragma unroll
   for (int n = 0; n < N; ++n) v[n] = 0.f;
@@ -369,8 +383,10 @@ __device__ __forceinline__ void group_sum(float (&v)[N], int G, float* red, int&
 
 constexpr int kRowThreads = 256;
 
+// The next rows are on their way while a group works on its rows: a group is one or a few
+// warps, too few per SM to hide the loads' latency by their number.
 template <typename T, int VEC, int EPT, int R>
-__global__ void __launch_bounds__(kRowThreads, 3) ln_rows_fwd_kernel(LnArgs a, int G) {
+__global__ void __launch_bounds__(kRowThreads, 2) ln_rows_fwd_kernel(LnArgs a, int G) {
   using Frag = RowFrag<T, VEC, EPT>;
   using P = typename Frag::P;
   extern __shared__ __align__(16) float ln_sm[];
@@ -378,18 +394,26 @@ __global__ void __launch_bounds__(kRowThreads, 3) ln_rows_fwd_kernel(LnArgs a, i
   int turn = 0;
   const int groups = blockDim.x / G, gi = threadIdx.x / G, gl = threadIdx.x - gi * G;
   const float rc = 1.f / (float)a.C;
+  const long long stride = (long long)gridDim.x * groups * R;
+  Frag next[R];
+  const auto load = [&](long long base) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long t = base + r * groups + gi;
+      next[r].load(static_cast<const T*>(a.x) + t * a.C, gl, G, a.C, t < a.tokens);
+    }
+  };
+  load((long long)blockIdx.x * groups * R);
   RowParam<T, VEC, EPT> w, b;
   w.fill(a.w, a.pdt, 1.f, ln_sm, gl, G, a.C);
   b.fill(a.b, a.pdt, 0.f, ln_sm + EPT * G, gl, G, a.C);
   if (!w.kRegs) __syncthreads();
-  for (long long base = (long long)blockIdx.x * groups * R; base < a.tokens; base += (long long)gridDim.x * groups * R) {
+  for (long long base = (long long)blockIdx.x * groups * R; base < a.tokens; base += stride) {
     Frag x[R];
     float s[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const long long t = base + r * groups + gi;
-      x[r].load(static_cast<const T*>(a.x) + t * a.C, gl, G, a.C, t < a.tokens);
-    }
+    for (int r = 0; r < R; ++r) x[r] = next[r];
+    if (base + stride < a.tokens) load(base + stride);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float2 sum = make_float2(0.f, 0.f);
@@ -455,24 +479,39 @@ __global__ void __launch_bounds__(kRowThreads, 2) ln_rows_bwd_kernel(LnArgs a, i
   int turn = 0;
   const int groups = blockDim.x / G, gi = threadIdx.x / G, gl = threadIdx.x - gi * G;
   const float rc = 1.f / (float)a.C;
+  constexpr bool kAhead = EPT <= 16;  // 32 elements' sums leave no registers for the next rows
+  const long long stride = (long long)gridDim.x * groups * R;
+  Frag xn[R], dn[R];
+  float2 stn[R];
+  const auto load = [&](long long base) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long t = base + r * groups + gi;
+      const bool in = t < a.tokens;
+      xn[r].load(static_cast<const T*>(a.x) + t * a.C, gl, G, a.C, in);
+      dn[r].load(static_cast<const T*>(a.dy) + t * a.C, gl, G, a.C, in);
+      stn[r] = in ? a.stats[t] : make_float2(0.f, 0.f);
+    }
+  };
+  if (kAhead) load((long long)blockIdx.x * groups * R);
   RowParam<T, VEC, EPT> w;
   w.fill(a.w, a.pdt, 1.f, ln_sm, gl, G, a.C);
   if (!w.kRegs) __syncthreads();
   float2 dw[EPT / 2], db[EPT / 2];
 #pragma unroll
   for (int i = 0; i < EPT / 2; ++i) dw[i] = db[i] = make_float2(0.f, 0.f);
-  for (long long base = (long long)blockIdx.x * groups * R; base < a.tokens; base += (long long)gridDim.x * groups * R) {
+  for (long long base = (long long)blockIdx.x * groups * R; base < a.tokens; base += stride) {
     Frag x[R], d[R];
     float2 st[R];
     float s[2 * R];
+    if (!kAhead) load(base);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const long long t = base + r * groups + gi;
-      const bool in = t < a.tokens;
-      x[r].load(static_cast<const T*>(a.x) + t * a.C, gl, G, a.C, in);
-      d[r].load(static_cast<const T*>(a.dy) + t * a.C, gl, G, a.C, in);
-      st[r] = in ? a.stats[t] : make_float2(0.f, 0.f);
+      x[r] = xn[r];
+      d[r] = dn[r];
+      st[r] = stn[r];
     }
+    if (kAhead && base + stride < a.tokens) load(base + stride);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float2 s1 = make_float2(0.f, 0.f), s2 = s1;
@@ -995,8 +1034,10 @@ struct LnPlan {
   long long units;  // CTA-sized pieces of work
 };
 
-// Rows: a power of two of threads with 8 elements each up to 256 columns, one warp with 16,
-// 24 or 32 up to 1024, then as many warps with 32 as the CTA has: 8192 columns.
+// Rows: a power of two of threads with 8 elements each up to 256 columns, whole warps with 16
+// up to 4096, then with 32 as many as the CTA has: 8192 columns.  (16 against 32 per thread:
+// 4096 x 4096 fp32 forward 25 us against 36, backward 44 against 69; 16384 x 1024 bf16
+// forward 17.8 against 16.8, backward 28 against 35.)
 LnPlan plan_rows(long long tokens, int C, int vec) {
   LnPlan p{};
   p.form = kAny;
@@ -1004,7 +1045,7 @@ LnPlan plan_rows(long long tokens, int C, int vec) {
   if (C > kRowThreads * (vec == 1 ? 8 : 32)) return p;
   p.form = kRows;
   p.vec = vec;
-  p.ept = vec == 1 || C <= 256 ? 8 : C <= 512 ? 16 : C <= 768 ? 24 : 32;
+  p.ept = vec == 1 || C <= 256 ? 8 : C <= kRowThreads * 16 ? 16 : 32;
   const int need = (C + p.ept - 1) / p.ept;
   p.G = 1;
   while (p.G < need && p.G < 32) p.G *= 2;
@@ -1069,7 +1110,7 @@ int launch_rows(const LnArgs& a, const LnPlan& p, bool bwd, int parts, cudaStrea
     auto kern = ln_rows_fwd_kernel<T, VEC, EPT, R>;
     const int st = ensure_smem(kern, 2 * param);
     if (st != MEDNEXT_OK) return st;
-    const long long cap = kSms * 3LL;  // resident by the launch bounds
+    const long long cap = kSms * 2LL;  // resident by the launch bounds
     kern<<<(unsigned)std::min((p.units + R - 1) / R, cap), p.threads, 2 * param, s>>>(a, p.G);
   } else {
     constexpr int RB = R > 2 ? 2 : 1;
@@ -1091,7 +1132,6 @@ int launch_rows_vec(const LnArgs& a, const LnPlan& p, bool bwd, int parts, cudaS
   if constexpr (VEC > 1) {
     if (p.ept == 16)
       return many ? launch_rows<T, VEC, 16, 2>(a, p, bwd, parts, s) : launch_rows<T, VEC, 16, 1>(a, p, bwd, parts, s);
-    if (p.ept == 24) return launch_rows<T, VEC, 24, 1>(a, p, bwd, parts, s);
     return launch_rows<T, VEC, 32, 1>(a, p, bwd, parts, s);
   }
   return MEDNEXT_ERR_UNSUPPORTED;  // not reached
