@@ -331,6 +331,86 @@ __device__ __forceinline__ void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint
       : "memory");
 }
 
+// The scaling and staged store of one warp's 32 accumulator lanes of a tile.  Fragment layout:
+// thread t has rows t / 4 + 8 i (i < 4) and column pairs 8 x + 2 (t % 4).
+template <typename T, bool TOKENS_A>
+struct StagedTile {
+  const I8GemmArgs& p;
+  float4* col;  // the warp's [16]: (scale, bias) of 32 columns' output channels or tokens
+  int lane, r0, sample, b0;
+  float2 rs[4];  // (scale, bias) of the rows
+
+  __device__ __forceinline__ void columns(int c0) {
+    const int c = b0 + c0 + lane;
+    reinterpret_cast<float2*>(col)[lane] =
+        c < p.b_rows ? make_float2(p.b_scale[c], TOKENS_A && p.bias != nullptr ? p.bias[c] : 0.f) : make_float2(0.f, 0.f);
+  }
+  // The constants of the rows and of the first columns: on their way while the product is
+  // computed.
+  __device__ __forceinline__ void prepare(int first) {
+    const float* a_scale = p.a_scale + (long long)sample * p.a_rows;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int row = r0 + (lane >> 2) + 8 * k;
+      rs[k] = row < p.a_rows ? make_float2(a_scale[row], !TOKENS_A && p.bias != nullptr ? p.bias[row] : 0.f)
+                             : make_float2(0.f, 0.f);
+    }
+    __syncwarp();
+    columns(first);
+  }
+  // t0: TMEM address of the warp's lanes, column 0; stg: two staging buffers; stored: stores
+  // so far by this warp.
+  __device__ __forceinline__ void store(const CUtensorMap* mY, uint32_t t0, int first, int next, uint8_t* stg,
+                                        int& stored) {
+    const int tc = lane & 3;
+    for (int c0 = first; c0 < p.bn && b0 + c0 < p.b_rows; c0 += next) {
+      uint32_t r[2][2][8];  // [16 rows][16 columns]
+      __syncwarp();         // the previous piece's constants are read
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          tmem_ld_16x256b_x2(t0 + (uint32_t)(c0 + 16 * x) + ((uint32_t)(16 * h) << 16), r[h][x]);
+      if (c0 > first) columns(c0);
+      uint8_t* buf = stg + (stored & 1) * kI8StageBytes;
+      if (stored >= 2 && lane == 0) bulk_wait_read<1>();  // the store from this buffer has read it
+      __syncwarp();
+      tmem_ld_wait();
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float4 k[2];  // (scale, bias) x 2 of the columns 16 x + 8 y + 2 tc
+#pragma unroll
+        for (int y = 0; y < 2; ++y) k[y] = col[8 * x + 4 * y + tc];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t q[4];
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {  // rows + 8 (m % 2), columns + 8 (m / 2)
+            const float2 v = make_float2((float)(int)r[h][x][2 * m], (float)(int)r[h][x][2 * m + 1]);
+            const float2 row = rs[2 * h + (m & 1)];
+            const float4 kc = k[m >> 1];
+            // (sum * token's scale) * channel's scale + bias
+            const float2 out =
+                TOKENS_A ? __ffma2_rn(__fmul2_rn(v, make_float2(row.x, row.x)), make_float2(kc.x, kc.z), make_float2(kc.y, kc.w))
+                         : __ffma2_rn(__fmul2_rn(v, make_float2(kc.x, kc.z)), make_float2(row.x, row.x), make_float2(row.y, row.y));
+            q[m] = pack2<T>(out);
+          }
+          const int R = 16 * x + 8 * (lane >> 4) + (lane & 7);  // the column this lane addresses
+          const int u = 2 * h + ((lane >> 3) & 1);              // its 16 bytes: 8 rows of A
+          stsm_x4_trans(smem_u32(buf) + (uint32_t)(R * 64 + (((u ^ (R >> 1)) & 3) << 4)), q);
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (r0 < p.a_rows) tma_store_3d(mY, buf, r0, b0 + c0, sample);
+        bulk_commit();
+      }
+      ++stored;
+    }
+  }
+};
+
 template <typename T, bool TOKENS_A, bool STAGED>
 __global__ void __launch_bounds__(kI8Threads, 1)
     i8_gemm_kernel(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUtensorMap mB,
@@ -434,12 +514,6 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       decode(i, sample, a0, b0);
       const int r0 = a0 + q4 * 32;  // this warp's first row of A
       const float* a_scale = p.a_scale + (long long)sample * p.a_rows;
-      // the constants of a column's output channel or token, shared by the warp's lanes
-      const auto columns = [&](int c0) {
-        const int c = b0 + c0 + lane;
-        col[lane] = c < p.b_rows ? make_float2(p.b_scale[c], TOKENS_A && p.bias != nullptr ? p.bias[c] : 0.f)
-                                 : make_float2(0.f, 0.f);
-      };
       // (false: a wait ran out, the warp leaves)
       const auto accumulated = [&] {
         if (!__all_sync(0xffffffffu, wait_or_abort(&sh.tfull[acc], (uint32_t)((i / p.accs) & 1), abort))) return false;
@@ -448,64 +522,10 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       };
       const uint32_t t0 = tmem + (uint32_t)(acc * p.bn) + ((uint32_t)(q4 * 32) << 16);
       if constexpr (STAGED) {
-        // fragment layout: thread t has rows t / 4 + 8 i (i < 4) and column pairs 8 x + 2 (t % 4)
-        const int tr = lane >> 2, tc = lane & 3;
-        float2 rs[4];  // (scale, bias) of the rows
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int row = r0 + tr + 8 * k;
-          rs[k] = row < p.a_rows ? make_float2(a_scale[row], !TOKENS_A && p.bias != nullptr ? p.bias[row] : 0.f)
-                                 : make_float2(0.f, 0.f);
-        }
-        __syncwarp();
-        columns(first);  // like the rows' constants, on their way while the product is computed
+        StagedTile<T, TOKENS_A> tile{p, sh.col[warp - 2], lane, r0, sample, b0, {}};
+        tile.prepare(first);
         if (!accumulated()) break;
-        for (int c0 = first; c0 < p.bn && b0 + c0 < p.b_rows; c0 += next) {
-          uint32_t r[2][2][8];  // [16 rows][16 columns]
-          __syncwarp();         // the previous piece's constants are read
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-              tmem_ld_16x256b_x2(t0 + (uint32_t)(c0 + 16 * x) + ((uint32_t)(16 * h) << 16), r[h][x]);
-          if (c0 > first) columns(c0);
-          uint8_t* buf = stg + (stored & 1) * kI8StageBytes;
-          if (stored >= 2 && lane == 0) bulk_wait_read<1>();  // the store from this buffer has read it
-          __syncwarp();
-          tmem_ld_wait();
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            float4 k[2];  // (scale, bias) x 2 of the columns 16 x + 8 y + 2 tc
-#pragma unroll
-            for (int y = 0; y < 2; ++y) k[y] = sh.col[warp - 2][8 * x + 4 * y + tc];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t q[4];
-#pragma unroll
-              for (int m = 0; m < 4; ++m) {  // rows + 8 (m % 2), columns + 8 (m / 2)
-                const float2 v = make_float2((float)(int)r[h][x][2 * m], (float)(int)r[h][x][2 * m + 1]);
-                const float2 row = rs[2 * h + (m & 1)];
-                const float4 kc = k[m >> 1];
-                // (sum * token's scale) * channel's scale + bias
-                const float2 out =
-                    TOKENS_A ? __ffma2_rn(__fmul2_rn(v, make_float2(row.x, row.x)), make_float2(kc.x, kc.z), make_float2(kc.y, kc.w))
-                             : __ffma2_rn(__fmul2_rn(v, make_float2(kc.x, kc.z)), make_float2(row.x, row.x), make_float2(row.y, row.y));
-                q[m] = pack2<T>(out);
-              }
-              const int R = 16 * x + 8 * (lane >> 4) + (lane & 7);  // the column this lane addresses
-              const int u = 2 * h + ((lane >> 3) & 1);              // its 16 bytes: 8 rows of A
-              stsm_x4_trans(smem_u32(buf) + (uint32_t)(R * 64 + (((u ^ (R >> 1)) & 3) << 4)), q);
-            }
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0 && r0 < p.a_rows) {
-            if (TOKENS_A) tma_store_3d(&mY, buf, r0, b0 + c0, sample);
-            else tma_store_3d(&mY, buf, r0, b0 + c0, 0);
-          }
-          if (lane == 0) bulk_commit();
-          ++stored;
-        }
+        tile.store(&mY, t0, first, next, stg, stored);
       } else {
         const int row = r0 + lane;
         const bool in = row < p.a_rows;
@@ -519,7 +539,9 @@ __global__ void __launch_bounds__(kI8Threads, 1)
           uint32_t r[32];
           __syncwarp();  // whole again, and the previous piece's constants are read
           tmem_ld32(t0 + (uint32_t)c0, r);
-          columns(c0);
+          const int c = b0 + c0 + lane;
+          col[lane] = c < p.b_rows ? make_float2(p.b_scale[c], TOKENS_A && p.bias != nullptr ? p.bias[c] : 0.f)
+                                   : make_float2(0.f, 0.f);
           __syncwarp();
           tmem_ld_wait();
           T* at = y + c0 * step;
@@ -548,6 +570,186 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, tmem_cols);
+}
+
+// ------------------------------ large products: two SMs per tile ------------------------------
+// One SM's 128 x 256 tile takes 48 KB of operands per 128 of K through the SM's load port, more
+// than the port's share of the tensor core's time (at 64 bytes a clock 768 clocks against 512).
+// A pair of CTAs (a cluster, tcgen05 cta_group::2) computes 256 x 256: each loads its 128 rows
+// of A and 128 of B's 256 rows, 32 KB, and the instruction reads both halves of B.
+//
+// The even CTA leads: its warp 1 issues the MMAs for both, whose accumulators lie in each
+// CTA's own TMEM.  Both CTAs' loads complete on the leader's barriers; a commit releases the
+// slot in both.  Epilogue warps of both release an accumulator at the leader.  The rest is as in the
+// kernel above; an accumulator is drained by all eight warps of its CTA.
+constexpr int kI8PairStages = 5;
+
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// A load into this CTA that completes on a barrier of the pair's leader.
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+      "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives at the same barrier of both CTAs once the MMAs issued so far are done.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+template <typename T, bool TOKENS_A>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
+    i8_gemm_pair_kernel(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUtensorMap mB,
+                        const __grid_constant__ CUtensorMap mY, I8GemmArgs p) {
+  extern __shared__ uint8_t i8_raw[];
+  __shared__ I8Shared sh;
+  constexpr int kHalf = kI8BM * kI8BK, kAccs = 2, kCols = 512;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)(blockIdx.x & 1);  // the cluster's CTAs are neighbours
+  uint8_t* ringA = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(i8_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* ringB = ringA + (size_t)kI8PairStages * kHalf;
+  uint8_t* stage = ringB + (size_t)kI8PairStages * kHalf;
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)),
+                 "r"((uint32_t)kCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kI8PairStages; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
+    }
+    for (int i = 0; i < kAccs; ++i) {
+      mbar_init(&sh.tfull[i], 1);
+      mbar_init(&sh.tempty[i], 2 * kI8EpiWarps);
+    }
+    mbar_init(&sh.drain, 1);
+    sh.abort = 0;
+    fence_mbarrier_init();
+    tma_prefetch_map(&mA);
+    tma_prefetch_map(&mB);
+    tma_prefetch_map(&mY);
+  }
+  grid_dependency_wait();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the pair's barriers are there
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem_base;
+  volatile int* abort = &sh.abort;
+  const int all = p.a_tiles * p.samples, tiles = all * p.b_tiles;
+  const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
+  const int mine = (tiles - pair + pairs - 1) / pairs;
+  const int kblocks = (p.K + kI8BK - 1) / kI8BK;
+  long long issued = 0;
+  const auto decode = [&](int i, int& sample, int& a0, int& b0) {  // a0: of this CTA's rows
+    const int t = pair + i * pairs;
+    const int ta = TOKENS_A ? t / p.b_tiles : t % all, tb = TOKENS_A ? t % p.b_tiles : t / all;
+    sample = ta / p.a_tiles;
+    a0 = (ta - sample * p.a_tiles) * (2 * kI8BM) + rank * kI8BM;
+    b0 = tb * p.bn;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int i = 0; i < mine && ok; ++i) {
+        int sample, a0, b0;
+        decode(i, sample, a0, b0);
+        for (int kb = 0; kb < kblocks; ++kb) {
+          const int st = (int)(issued % kI8PairStages);
+          const long long turn = issued / kI8PairStages;
+          if (turn > 0 && !(ok = wait_or_abort(&sh.empty[st], (uint32_t)((turn - 1) & 1), abort))) break;
+          if (rank == 0) mbar_arrive_expect_tx(&sh.full[st], 4 * kHalf);  // both CTAs' bytes
+          const uint32_t bar = cluster_addr(&sh.full[st], 0);
+          tma_load_3d_pair(ringA + (size_t)st * kHalf, &mA, bar, kb * kI8BK, a0, sample);
+          tma_load_3d_pair(ringB + (size_t)st * kHalf, &mB, bar, kb * kI8BK, b0 + rank * kI8BM, 0);
+          ++issued;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = make_idesc_i8(2 * kI8BM, 256);
+      long long q = 0;
+      bool ok = true;
+      for (int i = 0; i < mine && ok; ++i) {
+        const int acc = i % kAccs, turn = i / kAccs;
+        if (turn > 0 && !wait_or_abort(&sh.tempty[acc], (uint32_t)((turn - 1) & 1), abort)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(acc * 256);
+        for (int kb = 0; kb < kblocks; ++kb, ++q) {
+          const int st = (int)(q % kI8PairStages);
+          if (!(ok = wait_or_abort(&sh.full[st], (uint32_t)((q / kI8PairStages) & 1), abort))) break;
+          tc_fence_after();
+          const uint32_t sa = smem_u32(ringA + (size_t)st * kHalf), sb = smem_u32(ringB + (size_t)st * kHalf);
+          const int steps = min(kI8BK, p.K - kb * kI8BK + 31) / 32;
+          for (int ks = 0; ks < steps; ++ks)
+            mma_i8_pair(d, make_sw128_desc(sa + ks * 32, 16, 1024), make_sw128_desc(sb + ks * 32, 16, 1024), idesc,
+                        kb > 0 || ks > 0 ? 1u : 0u);
+          mma_commit_pair(&sh.empty[st]);
+        }
+        if (ok) mma_commit_pair(&sh.tfull[acc]);
+      }
+    }
+  } else {
+    const int q4 = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* stg = stage + (warp - 2) * 2 * kI8StageBytes;
+    int stored = 0;
+    for (int i = 0; i < mine; ++i) {
+      const int acc = i % kAccs;
+      int sample, a0, b0;
+      decode(i, sample, a0, b0);
+      StagedTile<T, TOKENS_A> tile{p, sh.col[warp - 2], lane, a0 + q4 * 32, sample, b0, {}};
+      tile.prepare(half * 32);
+      if (!__all_sync(0xffffffffu, wait_or_abort(&sh.tfull[acc], (uint32_t)((i / kAccs) & 1), abort))) break;
+      tc_fence_after();
+      tile.store(&mY, tmem + (uint32_t)(acc * 256) + ((uint32_t)(q4 * 32) << 16), half * 32, 64, stg, stored);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(cluster_addr(&sh.tempty[acc], 0));
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+  __syncthreads();
+  if (*abort && lane == 0 && rank == 0) {
+    if (warp == 0) drain_ring(sh.full, kI8PairStages, issued);
+    if (warp == 1) {
+      mma_commit_pair(&sh.drain);
+      mbar_wait(&sh.drain, 0);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA's memory is in use by the other any more
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kCols) : "memory");
 }
 
 // ------------------------------ narrow products in one kernel ------------------------------
@@ -918,6 +1120,30 @@ int num_sms() {
   return sms;
 }
 
+template <typename T>
+int launch_gemm_pair(I8GemmArgs p, bool tokens_a, const int8_t* a, long long a_pitch, const int8_t* b, long long b_pitch,
+                     int sms, cudaStream_t s) {
+  p.bn = 256;
+  p.a_tiles = (p.a_rows + 255) / 256;
+  p.b_tiles = (p.b_rows + 255) / 256;
+  const size_t smem = (size_t)kI8PairStages * 2 * kI8BM * kI8BK + kI8EpiWarps * 2 * kI8StageBytes + 1024;
+  CUtensorMap mA, mB, mY;
+  if (!tma::encode_rows_8bit(&mA, a, p.K, p.a_rows, p.samples, a_pitch, kI8BM) ||
+      !tma::encode_rows_8bit(&mB, b, p.K, p.b_rows, 1, b_pitch, kI8BM) ||
+      !tma::encode3<T>(&mY, p.y, p.a_rows, p.b_rows, p.samples, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)) {
+    note_cuda_error(cudaErrorInvalidValue);
+    return MEDNEXT_ERR_CUDA;
+  }
+  const long long tiles = (long long)p.a_tiles * p.samples * p.b_tiles;
+  const unsigned grid = 2 * (unsigned)std::min<long long>(tiles, sms / 2);
+  auto run = [&](auto kern) {
+    const int st = ensure_smem(kern, smem);
+    if (st != MEDNEXT_OK) return st;
+    return launch_dependent(kern, dim3(grid), dim3(kI8Threads), smem, s, mA, mB, mY, p);
+  };
+  return tokens_a ? run(i8_gemm_pair_kernel<T, true>) : run(i8_gemm_pair_kernel<T, false>);
+}
+
 // q: [outer * inner][q_pitch], w: [N][w_pitch]; y [outer, N, inner]
 template <typename T>
 int launch_gemm(const int8_t* q, const float* qs, long long q_pitch, const int8_t* w, const float* ws,
@@ -942,6 +1168,15 @@ int launch_gemm(const int8_t* q, const float* qs, long long q_pitch, const int8_
   while (p.bn > 32 && (p.bn / 2 >= p.b_rows || a_all * ((p.b_rows + p.bn - 1) / p.bn) < sms)) p.bn /= 2;
   p.b_tiles = (p.b_rows + p.bn - 1) / p.bn;
   if (a_all * p.b_tiles >= ((long long)1 << 31)) return MEDNEXT_ERR_BAD_SHAPE;
+  if constexpr (sizeof(T) == 2) {
+    // Pairs of SMs where both halves of the tiles are mostly full and every pair has one
+    // (32768 x 1024 -> 4096 bf16, the product alone: PAIRUS us against 149)
+    const long long pair_tiles = (long long)((p.a_rows + 255) / 256) * p.samples * ((p.b_rows + 255) / 256);
+    if (K >= 256 && p.a_rows % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0 && pair_tiles >= sms / 2 &&
+        p.a_rows > 128 && p.b_rows > 128)
+      return launch_gemm_pair<T>(p, tokens_a, tokens_a ? q : w, tokens_a ? q_pitch : w_pitch, tokens_a ? w : q,
+                                 tokens_a ? w_pitch : q_pitch, sms, s);
+  }
   p.accs = std::min(kI8MaxAcc, 512 / p.bn);
   p.share = p.accs < 4 || a_all * p.b_tiles <= sms;
   const int ring = kI8BM * kI8BK + p.bn * kI8BK, staging = kI8EpiWarps * 2 * kI8StageBytes;

@@ -253,3 +253,17 @@ def test_refusals():
             mx.int8_linear(*args, **kw)
     with pytest.raises(ValueError, match="131072"):
         mx.quantize_int8(torch.zeros((1, 131073), device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,k,n", [(2500, 300, 2056), (2305, 1024, 2304), (5000, 256, 1000), (1030, 2000, 4104)])
+def test_large_rows(t, k, n, dtype):
+    """Enough tiles for pairs of SMs; ragged last tiles in every direction."""
+    w, s, b = weights(n, k, seed=t)
+    check(activations((t, k), dtype, seed=k), w, s, b, -1)
+
+
+@pytest.mark.parametrize("outer,k,v,n", [(3, 300, 1000, 1800), (1, 512, 4096, 1300), (20, 260, 264, 1100), (2, 1000, 2568, 900)])
+def test_large_channels_first(outer, k, v, n):
+    w, s, b = weights(n, k, seed=v)
+    check(activations((outer, k, v), torch.bfloat16, seed=n), w, s, b, 1)
