@@ -71,9 +71,10 @@ struct DropRule {
 // before the generator runs.  VEC: every tensor starts on 16 bytes, and CTAs whose groups
 // are all whole move 16-byte vectors; RES: a residual is added.  One turn per CTA.
 //
-// Bound by instructions, not by bytes: about 5 per element for the generator (4 a round)
-// and 5 for the rest against 4 or 6 bytes of traffic.  U = 4 over 2 shares the round keys
-// and keeps 64 bytes of x in flight per thread.
+// 67.1 M bf16 elements: with a residual 61.7 us, 6.5 TB/s, bound by HBM; without 47.7 us, 5.6
+// TB/s, bound by instructions too: about 5 per element for the generator (4 a round) and 5
+// for the rest against 4 bytes of traffic.  One group per thread took 55.7 us: U = 4 shares
+// the round keys and keeps 64 bytes of x in flight.
 template <typename T, bool VEC, bool RES, int U>
 __global__ void __launch_bounds__(kDropThreads) dropout_kernel(DropArgs a) {
   uint64_t seed = a.seed, offset = a.offset;

@@ -38,12 +38,6 @@ __device__ __forceinline__ TokenScale token_scale(uint32_t max_bits) {
   s.inverse = max_bits >= 0x7f800000u ? 0.f : __fdiv_rn(127.f, m);
   return s;
 }
-__device__ __forceinline__ int8_t quantize(float v, TokenScale s) {
-  // |v| <= m_t, so the product is at most 127 (1 + 2^-23) and rounds into range; a token
-  // without a scale gives 0 (inverse 0; infinity * 0 = NaN converts to 0)
-  return (int8_t)__float2int_rn(__fmul_rn(v, s.inverse));
-}
-
 // ------------------------------ quantisation ------------------------------
 // rint(v * inverse) as the low byte of the sum with 1.5 * 2^23 (the sum's unit is 1, so its
 // rounding is the rint): two fp32 instructions in place of a conversion.  The product is
@@ -256,20 +250,44 @@ __global__ void __launch_bounds__(1024) i8_quantize_chan_kernel(const T* __restr
   }
 }
 
-// Rows of any alignment and width: one token per warp at a time, read twice.
+// Rows of any alignment and width: one token per warp at a time, four neighbouring values per
+// lane and step, so that their bytes are one store.  Up to 1024 values stay in registers;
+// longer rows are read again (from L1 / L2) to be scaled.
 template <typename T>
 __global__ void __launch_bounds__(256) i8_quantize_any_kernel(const T* __restrict__ x, int8_t* __restrict__ q,
                                                               float* __restrict__ scale, long long tokens, int K,
                                                               int pitch) {
+  constexpr int kSteps = 8;
   grid_dependents_go();
   const int lane = threadIdx.x & 31;
   for (long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); t < tokens; t += (long long)gridDim.x * 8) {
     const T* p = x + t * K;
+    const auto value = [&](int k) { return k < K ? to_acc<T>(p[k]) : 0.f; };
+    float v[kSteps][4];
     uint32_t m = 0;
-    for (int k = lane; k < K; k += 32) m = max(m, abs_bits(to_acc<T>(p[k])));
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[i][e] = value((i * 32 + lane) * 4 + e);
+        m = max(m, abs_bits(v[i][e]));
+      }
+    for (int k = (kSteps * 32 + lane) * 4; k < K; k += 128) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = max(m, abs_bits(value(k + e)));
+    }
     m = __reduce_max_sync(0xffffffffu, m);
     const TokenScale s = token_scale(m);
-    for (int k = lane; k < pitch; k += 32) q[t * pitch + k] = k < K ? quantize(to_acc<T>(p[k]), s) : (int8_t)0;
+    const uint32_t keep = m >= 0x7f800000u ? 0u : 0xffffffffu;
+    const auto store = [&](int k, float a, float b, float c, float d) {
+      const float2 f = scaled2(make_float2(a, b), s.inverse, s.inverse), g = scaled2(make_float2(c, d), s.inverse, s.inverse);
+      *reinterpret_cast<uint32_t*>(q + t * pitch + k) = low_bytes(f.x, f.y, g.x, g.y) & keep;
+    };
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+      if ((i * 32 + lane) * 4 < pitch) store((i * 32 + lane) * 4, v[i][0], v[i][1], v[i][2], v[i][3]);
+    for (int k = (kSteps * 32 + lane) * 4; k < pitch; k += 128)
+      store(k, value(k), value(k + 1), value(k + 2), value(k + 3));
     if (lane == 0) scale[t] = s.scale;
   }
 }
@@ -278,9 +296,12 @@ __global__ void __launch_bounds__(256) i8_quantize_any_kernel(const T* __restric
 // D[128 rows of A, bn rows of B] = A B^T in 8-bit integers with 32-bit sums
 // (tcgen05.mma kind::i8), both operands K-major rows under a 128-byte swizzle.
 //
-// Which operand is A goes by the output's layout, so that the 32 lanes of an accumulator
-// column lie side by side in y: channels-first output takes the tokens as A (lane =
-// voxel), rows take the weights as A (lane = output channel).
+// Which operand is A goes by the output's layout and by how it is stored.  Staged (y's rows are
+// whole 16-byte units): the accumulator's columns lie along y's rows, so A is the tokens for rows,
+// the weights for channels-first, and a lane's 128 bytes of columns are a row of a TMA store's
+// box.  (The other way round, lanes along y's rows, a warp's box has rows of 64 bytes, and
+// their rate was the bound: 127 us against 118 us for the product 32768 x 1024 -> 4096.)  Unstaged:
+// the lanes lie along y's rows, so that direct stores of one element per lane are coalesced.
 //
 // Persistent, warp-specialised: warp 0 issues the TMA loads (a ring of 128-byte K
 // blocks), warp 1 owns TMEM and issues the MMAs into two to four accumulators in turn, two
@@ -296,17 +317,27 @@ struct I8GemmArgs {
   const float* b_scale;  // of B's rows
   const float* bias;     // of the output channels, or NULL
   void* y;
-  int a_rows, b_rows, K;  // a_rows of one sample
+  int a_rows, b_rows, K;  // of one sample, where they are tokens
   int N;                  // output channels
   int bn, stages, accs;
   int share;  // the two groups share each tile
-  int a_tiles, samples, b_tiles;  // a_tiles of one sample
+  int a_tiles, b_tiles, samples;  // tiles of one sample
 };
 
-// Staged stores (16-bit y whose rows are whole 16-byte units): an epilogue warp turns its 32
-// lanes x 32 columns into rows of 64 bytes in shared memory (64-byte swizzle) and sends them
-// by TMA.  Two buffers per warp.
-constexpr int kI8StageBytes = 32 * 64;
+// The tile that a CTA (or pair) takes in its turn: neighbours share a tile of tokens and
+// differ in the output channels.
+struct I8Tile {
+  int sample, ta, tb;
+};
+template <bool TOKENS_A>
+__device__ __forceinline__ I8Tile i8_tile(const I8GemmArgs& p, int t) {
+  const int chans = TOKENS_A ? p.b_tiles : p.a_tiles, tokens = TOKENS_A ? p.a_tiles : p.b_tiles;
+  const int tok = t / chans, ch = t - tok * chans, sample = tok / tokens, tt = tok - sample * tokens;
+  return TOKENS_A ? I8Tile{sample, tt, ch} : I8Tile{sample, ch, tt};
+}
+
+// A staging buffer: an epilogue warp's 32 lanes, 128 bytes each (128-byte swizzle).
+constexpr int kI8StageBytes = 32 * 128;
 
 struct I8Shared {
   uint64_t full[kI8MaxStages], empty[kI8MaxStages];
@@ -314,7 +345,7 @@ struct I8Shared {
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
-  float4 col[kI8EpiWarps][16];  // (scale, bias) of an epilogue warp's 32 columns
+  float4 col[kI8EpiWarps][32];  // (scale, bias) of an epilogue warp's columns
 };
 
 // Instruction descriptor, kind::i8: signed 8-bit operands, K-major, 32-bit integer sums.
@@ -331,82 +362,69 @@ __device__ __forceinline__ void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint
       : "memory");
 }
 
-// The scaling and staged store of one warp's 32 accumulator lanes of a tile.  Fragment layout:
-// thread t has rows t / 4 + 8 i (i < 4) and column pairs 8 x + 2 (t % 4).
+// The scaling and staged store of one warp's 32 accumulator lanes of a tile, 128 bytes of
+// columns at a time.
 template <typename T, bool TOKENS_A>
 struct StagedTile {
+  static constexpr int kCols = 128 / (int)sizeof(T);
   const I8GemmArgs& p;
-  float4* col;  // the warp's [16]: (scale, bias) of 32 columns' output channels or tokens
+  float4* col;  // the warp's [kCols / 2]: two columns' scales, and biases where they are output channels
   int lane, r0, sample, b0;
-  float2 rs[4];  // (scale, bias) of the rows
+  float scale, bias;  // of the lane's row
 
+  // the constants of kCols columns: two per lane (kCols = 64) or one of each pair's lanes
   __device__ __forceinline__ void columns(int c0) {
-    const int c = b0 + c0 + lane;
-    reinterpret_cast<float2*>(col)[lane] =
-        c < p.b_rows ? make_float2(p.b_scale[c], TOKENS_A && p.bias != nullptr ? p.bias[c] : 0.f) : make_float2(0.f, 0.f);
+    const float* b_scale = p.b_scale + (TOKENS_A ? 0LL : (long long)sample * p.b_rows);
+    const int c = b0 + c0 + 2 * lane;
+    if (2 * lane >= kCols) return;
+    const bool in0 = c < p.b_rows, in1 = c + 1 < p.b_rows, biased = TOKENS_A && p.bias != nullptr;
+    col[lane] = make_float4(in0 ? b_scale[c] : 0.f, in1 ? b_scale[c + 1] : 0.f, in0 && biased ? p.bias[c] : 0.f,
+                            in1 && biased ? p.bias[c + 1] : 0.f);
   }
-  // The constants of the rows and of the first columns: on their way while the product is
+  // The constants of the row and of the first columns: on their way while the product is
   // computed.
   __device__ __forceinline__ void prepare(int first) {
-    const float* a_scale = p.a_scale + (long long)sample * p.a_rows;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int row = r0 + (lane >> 2) + 8 * k;
-      rs[k] = row < p.a_rows ? make_float2(a_scale[row], !TOKENS_A && p.bias != nullptr ? p.bias[row] : 0.f)
-                             : make_float2(0.f, 0.f);
-    }
+    const int row = r0 + lane;
+    const bool in = row < p.a_rows;
+    scale = in ? p.a_scale[(TOKENS_A ? (long long)sample * p.a_rows : 0LL) + row] : 0.f;
+    bias = in && !TOKENS_A && p.bias != nullptr ? p.bias[row] : 0.f;
     __syncwarp();
     columns(first);
   }
-  // t0: TMEM address of the warp's lanes, column 0; stg: two staging buffers; stored: stores
-  // so far by this warp.
-  __device__ __forceinline__ void store(const CUtensorMap* mY, uint32_t t0, int first, int next, uint8_t* stg,
-                                        int& stored) {
-    const int tc = lane & 3;
+  // t0: TMEM address of the warp's lanes, column 0; stg: the warp's staging buffer.
+  __device__ __forceinline__ void store(const CUtensorMap* mY, uint32_t t0, int first, int next, uint8_t* stg) {
     for (int c0 = first; c0 < p.bn && b0 + c0 < p.b_rows; c0 += next) {
-      uint32_t r[2][2][8];  // [16 rows][16 columns]
-      __syncwarp();         // the previous piece's constants are read
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          tmem_ld_16x256b_x2(t0 + (uint32_t)(c0 + 16 * x) + ((uint32_t)(16 * h) << 16), r[h][x]);
+      __syncwarp();  // the previous piece's constants are read
       if (c0 > first) columns(c0);
-      uint8_t* buf = stg + (stored & 1) * kI8StageBytes;
-      if (stored >= 2 && lane == 0) bulk_wait_read<1>();  // the store from this buffer has read it
+      uint32_t r[kCols / 32][32];
+#pragma unroll
+      for (int h = 0; h < kCols / 32; ++h) tmem_ld32(t0 + (uint32_t)(c0 + 32 * h), r[h]);
+      if (lane == 0) bulk_wait_read<0>();  // the last store has read the buffer
       __syncwarp();
       tmem_ld_wait();
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float4 k[2];  // (scale, bias) x 2 of the columns 16 x + 8 y + 2 tc
+      for (int h = 0; h < kCols / 32; ++h) {
+        float2 out[16];
 #pragma unroll
-        for (int y = 0; y < 2; ++y) k[y] = col[8 * x + 4 * y + tc];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t q[4];
-#pragma unroll
-          for (int m = 0; m < 4; ++m) {  // rows + 8 (m % 2), columns + 8 (m / 2)
-            const float2 v = make_float2((float)(int)r[h][x][2 * m], (float)(int)r[h][x][2 * m + 1]);
-            const float2 row = rs[2 * h + (m & 1)];
-            const float4 kc = k[m >> 1];
-            // (sum * token's scale) * channel's scale + bias
-            const float2 out =
-                TOKENS_A ? __ffma2_rn(__fmul2_rn(v, make_float2(row.x, row.x)), make_float2(kc.x, kc.z), make_float2(kc.y, kc.w))
-                         : __ffma2_rn(__fmul2_rn(v, make_float2(kc.x, kc.z)), make_float2(row.x, row.x), make_float2(row.y, row.y));
-            q[m] = pack2<T>(out);
-          }
-          const int R = 16 * x + 8 * (lane >> 4) + (lane & 7);  // the column this lane addresses
-          const int u = 2 * h + ((lane >> 3) & 1);              // its 16 bytes: 8 rows of A
-          stsm_x4_trans(smem_u32(buf) + (uint32_t)(R * 64 + (((u ^ (R >> 1)) & 3) << 4)), q);
+        for (int j = 0; j < 16; ++j) {
+          const float4 k = col[16 * h + j];
+          const float2 v = make_float2((float)(int)r[h][2 * j], (float)(int)r[h][2 * j + 1]);
+          // (sum * token's scale) * channel's scale + bias
+          out[j] = TOKENS_A ? __ffma2_rn(__fmul2_rn(v, make_float2(scale, scale)), make_float2(k.x, k.y), make_float2(k.z, k.w))
+                            : __ffma2_rn(__fmul2_rn(v, make_float2(k.x, k.y)), make_float2(scale, scale), make_float2(bias, bias));
         }
+        const float* f = reinterpret_cast<const float*>(out);
+        constexpr int E = 16 / sizeof(T);
+#pragma unroll
+        for (int u = 0; u < 32 / E; ++u)
+          *reinterpret_cast<uint4*>(stg + lane * 128 + (((h * (32 / E) + u) ^ (lane & 7)) << 4)) = pack16<T>(f + u * E);
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) {
-        if (r0 < p.a_rows) tma_store_3d(mY, buf, r0, b0 + c0, sample);
+        if (r0 < p.a_rows) tma_store_3d(mY, stg, b0 + c0, r0, sample);
         bulk_commit();
       }
-      ++stored;
     }
   }
 };
@@ -447,17 +465,15 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   tc_fence_after();
   const uint32_t tmem = sh.tmem_base;
   volatile int* abort = &sh.abort;
-  const int tiles = p.a_tiles * p.samples * p.b_tiles;
+  const int tiles = p.a_tiles * p.b_tiles * p.samples;
   const int mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
   const int kblocks = (p.K + kI8BK - 1) / kI8BK;
   long long issued = 0;
-  // neighbouring CTAs share a tile of tokens and differ in the output channels
   const auto decode = [&](int i, int& sample, int& a0, int& b0) {
-    const int t = (int)blockIdx.x + i * (int)gridDim.x, all = p.a_tiles * p.samples;
-    const int ta = TOKENS_A ? t / p.b_tiles : t % all, tb = TOKENS_A ? t % p.b_tiles : t / all;
-    sample = ta / p.a_tiles;
-    a0 = (ta - sample * p.a_tiles) * kI8BM;
-    b0 = tb * p.bn;
+    const I8Tile t = i8_tile<TOKENS_A>(p, (int)blockIdx.x + i * (int)gridDim.x);
+    sample = t.sample;
+    a0 = t.ta * kI8BM;
+    b0 = t.tb * p.bn;
   };
 
   if (warp == 0) {
@@ -471,8 +487,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
           const long long turn = issued / p.stages;
           if (turn > 0 && !(ok = wait_or_abort(&sh.empty[st], (uint32_t)((turn - 1) & 1), abort))) break;
           mbar_arrive_expect_tx(&sh.full[st], (uint32_t)(kI8BM * kI8BK + b_bytes));
-          tma_load_3d(ringA + (size_t)st * (kI8BM * kI8BK), &mA, &sh.full[st], kb * kI8BK, a0, sample);
-          tma_load_3d(ringB + (size_t)st * b_bytes, &mB, &sh.full[st], kb * kI8BK, b0, 0);
+          tma_load_3d(ringA + (size_t)st * (kI8BM * kI8BK), &mA, &sh.full[st], kb * kI8BK, a0, TOKENS_A ? sample : 0);
+          tma_load_3d(ringB + (size_t)st * b_bytes, &mB, &sh.full[st], kb * kI8BK, b0, TOKENS_A ? 0 : sample);
           ++issued;
         }
       }
@@ -502,18 +518,17 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       }
     }
   } else {
-    // accumulator lanes 32 * (warp % 4) ..; 32 columns at a time
+    // accumulator lanes 32 * (warp % 4) ..; 128 bytes or 32 columns at a time
     const int q4 = warp & 3, half = (warp - 2) >> 2;
-    const int first = p.share ? half * 32 : 0, next = p.share ? 64 : 32;
+    constexpr int kPiece = STAGED ? 128 / (int)sizeof(T) : 32;
+    const int first = p.share ? half * kPiece : 0, next = p.share ? 2 * kPiece : kPiece;
     float2* col = reinterpret_cast<float2*>(sh.col[warp - 2]);
-    uint8_t* stg = stage + (warp - 2) * 2 * kI8StageBytes;
-    int stored = 0;
+    uint8_t* stg = stage + (warp - 2) * kI8StageBytes;
     for (int i = p.share ? 0 : half; i < mine; i += p.share ? 1 : 2) {
       const int acc = i % p.accs;
       int sample, a0, b0;
       decode(i, sample, a0, b0);
       const int r0 = a0 + q4 * 32;  // this warp's first row of A
-      const float* a_scale = p.a_scale + (long long)sample * p.a_rows;
       // (false: a wait ran out, the warp leaves)
       const auto accumulated = [&] {
         if (!__all_sync(0xffffffffu, wait_or_abort(&sh.tfull[acc], (uint32_t)((i / p.accs) & 1), abort))) return false;
@@ -522,14 +537,15 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       };
       const uint32_t t0 = tmem + (uint32_t)(acc * p.bn) + ((uint32_t)(q4 * 32) << 16);
       if constexpr (STAGED) {
-        StagedTile<T, TOKENS_A> tile{p, sh.col[warp - 2], lane, r0, sample, b0, {}};
+        StagedTile<T, TOKENS_A> tile{p, sh.col[warp - 2], lane, r0, sample, b0, 0.f, 0.f};
         tile.prepare(first);
         if (!accumulated()) break;
-        tile.store(&mY, t0, first, next, stg, stored);
+        tile.store(&mY, t0, first, next, stg);
       } else {
         const int row = r0 + lane;
         const bool in = row < p.a_rows;
-        const float row_scale = in ? a_scale[row] : 0.f;
+        // TOKENS_A goes with channels-first here
+        const float row_scale = in ? p.a_scale[(TOKENS_A ? (long long)sample * p.a_rows : 0LL) + row] : 0.f;
         const float row_bias = !TOKENS_A && in && p.bias != nullptr ? p.bias[row] : 0.f;
         const long long step = TOKENS_A ? p.a_rows : p.N;  // of y, from one column to the next
         T* y = static_cast<T*>(p.y) + row +
@@ -582,6 +598,10 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 // CTA's own TMEM.  Both CTAs' loads complete on the leader's barriers; a commit releases the
 // slot in both.  Epilogue warps of both release an accumulator at the leader.  The rest is as in the
 // kernel above; an accumulator is drained by all eight warps of its CTA.
+//
+// 8192 x 4096 -> 4096 bf16: 98 us in the product, 2.8 POP/s (one SM per tile: 131 us);
+// 32768 x 1024 -> 4096: 118 us, 2.3 POP/s, the epilogue and its 268 MB of output sharing the
+// bound.
 constexpr int kI8PairStages = 5;
 
 __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
@@ -663,17 +683,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
   tc_fence_after();
   const uint32_t tmem = sh.tmem_base;
   volatile int* abort = &sh.abort;
-  const int all = p.a_tiles * p.samples, tiles = all * p.b_tiles;
+  const int tiles = p.a_tiles * p.b_tiles * p.samples;
   const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
   const int mine = (tiles - pair + pairs - 1) / pairs;
   const int kblocks = (p.K + kI8BK - 1) / kI8BK;
   long long issued = 0;
   const auto decode = [&](int i, int& sample, int& a0, int& b0) {  // a0: of this CTA's rows
-    const int t = pair + i * pairs;
-    const int ta = TOKENS_A ? t / p.b_tiles : t % all, tb = TOKENS_A ? t % p.b_tiles : t / all;
-    sample = ta / p.a_tiles;
-    a0 = (ta - sample * p.a_tiles) * (2 * kI8BM) + rank * kI8BM;
-    b0 = tb * p.bn;
+    const I8Tile t = i8_tile<TOKENS_A>(p, pair + i * pairs);
+    sample = t.sample;
+    a0 = t.ta * (2 * kI8BM) + rank * kI8BM;
+    b0 = t.tb * 256;
   };
 
   if (warp == 0) {
@@ -688,8 +707,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
           if (turn > 0 && !(ok = wait_or_abort(&sh.empty[st], (uint32_t)((turn - 1) & 1), abort))) break;
           if (rank == 0) mbar_arrive_expect_tx(&sh.full[st], 4 * kHalf);  // both CTAs' bytes
           const uint32_t bar = cluster_addr(&sh.full[st], 0);
-          tma_load_3d_pair(ringA + (size_t)st * kHalf, &mA, bar, kb * kI8BK, a0, sample);
-          tma_load_3d_pair(ringB + (size_t)st * kHalf, &mB, bar, kb * kI8BK, b0 + rank * kI8BM, 0);
+          tma_load_3d_pair(ringA + (size_t)st * kHalf, &mA, bar, kb * kI8BK, a0, TOKENS_A ? sample : 0);
+          tma_load_3d_pair(ringB + (size_t)st * kHalf, &mB, bar, kb * kI8BK, b0 + rank * kI8BM, TOKENS_A ? 0 : sample);
           ++issued;
         }
       }
@@ -720,17 +739,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
     }
   } else {
     const int q4 = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* stg = stage + (warp - 2) * 2 * kI8StageBytes;
-    int stored = 0;
+    constexpr int kPiece = 128 / (int)sizeof(T);
+    uint8_t* stg = stage + (warp - 2) * kI8StageBytes;
     for (int i = 0; i < mine; ++i) {
       const int acc = i % kAccs;
       int sample, a0, b0;
       decode(i, sample, a0, b0);
-      StagedTile<T, TOKENS_A> tile{p, sh.col[warp - 2], lane, a0 + q4 * 32, sample, b0, {}};
-      tile.prepare(half * 32);
+      StagedTile<T, TOKENS_A> tile{p, sh.col[warp - 2], lane, a0 + q4 * 32, sample, b0, 0.f, 0.f};
+      tile.prepare(half * kPiece);
       if (!__all_sync(0xffffffffu, wait_or_abort(&sh.tfull[acc], (uint32_t)((i / kAccs) & 1), abort))) break;
       tc_fence_after();
-      tile.store(&mY, tmem + (uint32_t)(acc * 256) + ((uint32_t)(q4 * 32) << 16), half * 32, 64, stg, stored);
+      tile.store(&mY, tmem + (uint32_t)(acc * 256) + ((uint32_t)(q4 * 32) << 16), half * kPiece, 2 * kPiece, stg);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(cluster_addr(&sh.tempty[acc], 0));
@@ -1120,28 +1139,15 @@ int num_sms() {
   return sms;
 }
 
+// Tensor maps of a product's operands (the tokens' with a matrix per sample) and, staged, of y.
 template <typename T>
-int launch_gemm_pair(I8GemmArgs p, bool tokens_a, const int8_t* a, long long a_pitch, const int8_t* b, long long b_pitch,
-                     int sms, cudaStream_t s) {
-  p.bn = 256;
-  p.a_tiles = (p.a_rows + 255) / 256;
-  p.b_tiles = (p.b_rows + 255) / 256;
-  const size_t smem = (size_t)kI8PairStages * 2 * kI8BM * kI8BK + kI8EpiWarps * 2 * kI8StageBytes + 1024;
-  CUtensorMap mA, mB, mY;
-  if (!tma::encode_rows_8bit(&mA, a, p.K, p.a_rows, p.samples, a_pitch, kI8BM) ||
-      !tma::encode_rows_8bit(&mB, b, p.K, p.b_rows, 1, b_pitch, kI8BM) ||
-      !tma::encode3<T>(&mY, p.y, p.a_rows, p.b_rows, p.samples, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)) {
-    note_cuda_error(cudaErrorInvalidValue);
-    return MEDNEXT_ERR_CUDA;
-  }
-  const long long tiles = (long long)p.a_tiles * p.samples * p.b_tiles;
-  const unsigned grid = 2 * (unsigned)std::min<long long>(tiles, sms / 2);
-  auto run = [&](auto kern) {
-    const int st = ensure_smem(kern, smem);
-    if (st != MEDNEXT_OK) return st;
-    return launch_dependent(kern, dim3(grid), dim3(kI8Threads), smem, s, mA, mB, mY, p);
-  };
-  return tokens_a ? run(i8_gemm_pair_kernel<T, true>) : run(i8_gemm_pair_kernel<T, false>);
+bool i8_maps(const I8GemmArgs& p, bool tokens_a, bool staged, const int8_t* a, long long a_pitch, const int8_t* b,
+             long long b_pitch, uint32_t b_box, CUtensorMap* mA, CUtensorMap* mB, CUtensorMap* mY) {
+  memset(mY, 0, sizeof(*mY));
+  return tma::encode_rows_8bit(mA, a, p.K, p.a_rows, tokens_a ? p.samples : 1, a_pitch, kI8BM) &&
+         tma::encode_rows_8bit(mB, b, p.K, p.b_rows, tokens_a ? 1 : p.samples, b_pitch, b_box) &&
+         (!staged || tma::encode3<T>(mY, p.y, p.b_rows, p.a_rows, p.samples, 128 / sizeof(T), 32,
+                                     CU_TENSOR_MAP_SWIZZLE_128B));
 }
 
 // q: [outer * inner][q_pitch], w: [N][w_pitch]; y [outer, N, inner]
@@ -1149,62 +1155,69 @@ template <typename T>
 int launch_gemm(const int8_t* q, const float* qs, long long q_pitch, const int8_t* w, const float* ws,
                 long long w_pitch, const float* bias, void* y, long long outer, long long inner, int K, int N,
                 cudaStream_t s) {
-  const bool tokens_a = inner > 1;
+  const bool chan = inner > 1;
+  const long long tokens = chan ? inner : outer;  // of a sample
+  const bool staged = (chan ? inner : N) % (16 / (long long)sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+  const bool tokens_a = staged != chan;
+  const int8_t *a = tokens_a ? q : w, *b = tokens_a ? w : q;
+  const long long a_pitch = tokens_a ? q_pitch : w_pitch, b_pitch = tokens_a ? w_pitch : q_pitch;
   I8GemmArgs p{};
   p.a_scale = tokens_a ? qs : ws;
   p.b_scale = tokens_a ? ws : qs;
   p.bias = bias;
   p.y = y;
-  p.a_rows = tokens_a ? (int)inner : N;
-  p.samples = tokens_a ? (int)outer : 1;
-  p.b_rows = tokens_a ? N : (int)outer;
+  p.a_rows = tokens_a ? (int)tokens : N;
+  p.b_rows = tokens_a ? N : (int)tokens;
+  p.samples = chan ? (int)outer : 1;
   p.K = K;
   p.N = N;
-  p.a_tiles = (p.a_rows + kI8BM - 1) / kI8BM;
   const int sms = num_sms();
-  const long long a_all = (long long)p.a_tiles * p.samples;
-  // the widest B tile that still gives every SM a tile, at most what B fills
-  p.bn = 256;
-  while (p.bn > 32 && (p.bn / 2 >= p.b_rows || a_all * ((p.b_rows + p.bn - 1) / p.bn) < sms)) p.bn /= 2;
-  p.b_tiles = (p.b_rows + p.bn - 1) / p.bn;
-  if (a_all * p.b_tiles >= ((long long)1 << 31)) return MEDNEXT_ERR_BAD_SHAPE;
-  if constexpr (sizeof(T) == 2) {
-    // Pairs of SMs where both halves of the tiles are mostly full and every pair has one
-    // (32768 x 1024 -> 4096 bf16, the product alone: PAIRUS us against 149)
-    const long long pair_tiles = (long long)((p.a_rows + 255) / 256) * p.samples * ((p.b_rows + 255) / 256);
-    if (K >= 256 && p.a_rows % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0 && pair_tiles >= sms / 2 &&
-        p.a_rows > 128 && p.b_rows > 128)
-      return launch_gemm_pair<T>(p, tokens_a, tokens_a ? q : w, tokens_a ? q_pitch : w_pitch, tokens_a ? w : q,
-                                 tokens_a ? w_pitch : q_pitch, sms, s);
-  }
-  p.accs = std::min(kI8MaxAcc, 512 / p.bn);
-  p.share = p.accs < 4 || a_all * p.b_tiles <= sms;
-  const int ring = kI8BM * kI8BK + p.bn * kI8BK, staging = kI8EpiWarps * 2 * kI8StageBytes;
-  p.stages = std::min(kI8MaxStages, (216 * 1024 - staging) / ring);
-  const size_t smem = (size_t)p.stages * ring + staging + 1024;
   CUtensorMap mA, mB, mY;
-  memset(&mY, 0, sizeof(mY));
-  bool staged = false;
-  bool ok = tma::encode_rows_8bit(&mA, tokens_a ? q : w, K, p.a_rows, p.samples, tokens_a ? q_pitch : w_pitch, kI8BM) &&
-            tma::encode_rows_8bit(&mB, tokens_a ? w : q, K, p.b_rows, 1, tokens_a ? w_pitch : q_pitch, p.bn);
-  if constexpr (sizeof(T) == 2) {
-    staged = p.a_rows % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
-    if (staged)
-      ok = ok && tma::encode3<T>(&mY, y, p.a_rows, p.b_rows, p.samples, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
-  }
-  if (!ok) {
+  const auto no_map = [] {
     note_cuda_error(cudaErrorInvalidValue);
-    return MEDNEXT_ERR_CUDA;
-  }
-  const unsigned grid = (unsigned)std::min<long long>(a_all * p.b_tiles, sms);
-  auto run = [&](auto kern) {
+    return (int)MEDNEXT_ERR_CUDA;
+  };
+  const auto run = [&](auto kern, unsigned grid, size_t smem) {
     const int st = ensure_smem(kern, smem);
     if (st != MEDNEXT_OK) return st;
     return launch_dependent(kern, dim3(grid), dim3(kI8Threads), smem, s, mA, mB, mY, p);
   };
-  if constexpr (sizeof(T) == 2)
-    if (staged) return tokens_a ? run(i8_gemm_kernel<T, true, true>) : run(i8_gemm_kernel<T, false, true>);
-  return tokens_a ? run(i8_gemm_kernel<T, true, false>) : run(i8_gemm_kernel<T, false, false>);
+  const int staging = staged ? kI8EpiWarps * kI8StageBytes : 0;
+
+  // Pairs of SMs where both halves of the tiles are mostly full and every pair has one
+  // (32768 x 1024 -> 4096 bf16, the product alone: 118 us against 149).
+  const long long pair_tiles = (long long)((p.a_rows + 255) / 256) * ((p.b_rows + 255) / 256) * p.samples;
+  if (staged && K >= 256 && p.a_rows > 128 && p.b_rows > 128 && pair_tiles >= sms / 2) {
+    if (pair_tiles >= ((long long)1 << 31)) return MEDNEXT_ERR_BAD_SHAPE;
+    p.bn = 256;
+    p.a_tiles = (p.a_rows + 255) / 256;
+    p.b_tiles = (p.b_rows + 255) / 256;
+    if (!i8_maps<T>(p, tokens_a, staged, a, a_pitch, b, b_pitch, kI8BM, &mA, &mB, &mY)) return no_map();
+    const size_t smem = (size_t)kI8PairStages * 2 * kI8BM * kI8BK + staging + 1024;
+    const unsigned grid = 2 * (unsigned)std::min<long long>(pair_tiles, sms / 2);
+    return tokens_a ? run(i8_gemm_pair_kernel<T, true>, grid, smem) : run(i8_gemm_pair_kernel<T, false>, grid, smem);
+  }
+
+  p.a_tiles = (p.a_rows + kI8BM - 1) / kI8BM;
+  const long long a_all = (long long)p.a_tiles * p.samples;
+  // the widest B tile that still gives every SM a tile, at most what B fills; at least a
+  // staged store's columns
+  const int least = staged ? std::max(32, 128 / (int)sizeof(T)) : 32;
+  p.bn = 256;
+  while (p.bn > least && (p.bn / 2 >= p.b_rows || a_all * ((p.b_rows + p.bn - 1) / p.bn) < sms)) p.bn /= 2;
+  p.b_tiles = (p.b_rows + p.bn - 1) / p.bn;
+  const long long tiles = a_all * p.b_tiles;
+  if (tiles >= ((long long)1 << 31)) return MEDNEXT_ERR_BAD_SHAPE;
+  p.accs = std::min(kI8MaxAcc, 512 / p.bn);
+  p.share = p.accs < 4 || tiles <= sms;
+  const int ring = kI8BM * kI8BK + p.bn * kI8BK;
+  p.stages = std::min(kI8MaxStages, (216 * 1024 - staging) / ring);
+  if (!i8_maps<T>(p, tokens_a, staged, a, a_pitch, b, b_pitch, p.bn, &mA, &mB, &mY)) return no_map();
+  const size_t smem = (size_t)p.stages * ring + staging + 1024;
+  const unsigned grid = (unsigned)std::min<long long>(tiles, sms);
+  if (staged)
+    return tokens_a ? run(i8_gemm_kernel<T, true, true>, grid, smem) : run(i8_gemm_kernel<T, false, true>, grid, smem);
+  return tokens_a ? run(i8_gemm_kernel<T, true, false>, grid, smem) : run(i8_gemm_kernel<T, false, false>, grid, smem);
 }
 
 long long pitch16(int64_t k) { return (k + 15) / 16 * 16; }

@@ -145,12 +145,39 @@ def _grn_cases(dev: torch.device) -> dict[str, tuple]:
     }
 
 
+def _mixer_cases(dev: torch.device) -> dict[str, tuple]:
+    """Layer norm, dropout and 8-bit products on level 0 and on wide rows (bf16)."""
+    from .drop import dropout
+    from .norm import _backward, _forward, layer_norm
+    from .quant import int8_linear, quantize_int8
+
+    bf = torch.bfloat16
+    x, dy = (torch.randn((1, C, V), device=dev).to(bf) for _ in range(2))
+    g, b = torch.ones(C, device=dev), torch.zeros(C, device=dev)
+    stats = _forward(x, g, b, 1e-6, 1, True)[1]
+    rng = torch.tensor([1, 2], device=dev)
+    q, s = quantize_int8(torch.randn((RC, C), device=dev))
+    rows = torch.randn((32768, 1024), device=dev).to(bf)
+    qr, sr = quantize_int8(torch.randn((4096, 1024), device=dev))
+    nbytes = 2 * C * V
+    return {
+        "mixer layer norm fwd C32 128^3": (lambda: layer_norm(x, g, b, dim=1), 2 * nbytes),
+        "mixer layer norm bwd C32 128^3": (lambda: _backward(dy, x, stats, g, b, 1, True), 3 * nbytes),
+        "mixer dropout + residual C32 128^3": (lambda: dropout(x, 0.1, rng, residual=dy), 3 * nbytes),
+        "mixer dropout C32 128^3": (lambda: dropout(x, 0.1, rng), 2 * nbytes),
+        "mixer int8 32 -> 64 128^3": (lambda: int8_linear(x, q, s, dim=1), 3 * nbytes),
+        "mixer int8 32768 x 1024 -> 4096": (lambda: int8_linear(rows, qr, sr), 2 * 32768 * 5120 + 4096 * 1024),
+    }
+
+
 def run(patterns: list[str], reps: int = 10, warmup: int = 3) -> dict[str, dict]:
     dev = torch.device("cuda", torch.cuda.current_device())
     results = {}
     cases = _cases(dev)
     if not patterns or any("grn" in p for p in patterns):
         cases.update(_grn_cases(dev))
+    if not patterns or any("mixer" in p for p in patterns):
+        cases.update(_mixer_cases(dev))
     for name, (fn, nbytes) in cases.items():
         if patterns and not any(p in name for p in patterns):
             continue

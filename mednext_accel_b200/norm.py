@@ -20,6 +20,7 @@ about 18 us on the host, the autograd function's 6 us.
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 
 import torch
 from torch import Tensor, nn
@@ -71,10 +72,15 @@ def _forward(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float, 
              want_stats: bool) -> tuple[Tensor, Tensor | None]:
     outer, c, inner = axis_sizes(x, dim)
     y = torch.empty_like(x)
-    stats = torch.empty((outer * inner, 2), dtype=torch.float32, device=x.device) if want_stats else None
+    stats = x.new_empty((outer * inner, 2), dtype=torch.float32) if want_stats else None
     nat.launch("mednext_ln_fwd", x, x.data_ptr(), nat.ptr(weight), nat.ptr(bias), y.data_ptr(), nat.ptr(stats),
                outer, c, inner, eps, nat.dtype_code(x.dtype), _param_code(x, weight, bias))
     return y, stats
+
+
+@lru_cache(maxsize=1024)
+def _workspace_size(outer: int, c: int, inner: int, code: int) -> int:
+    return nat.load().mednext_ln_bwd_workspace_size(outer, c, inner, code)
 
 
 def _backward(dy: Tensor, x: Tensor, stats: Tensor, weight: Tensor | None, bias: Tensor | None, dim: int,
@@ -86,8 +92,8 @@ def _backward(dy: Tensor, x: Tensor, stats: Tensor, weight: Tensor | None, bias:
     db = torch.empty_like(bias) if want_params and bias is not None else None
     ws, nbytes = None, 0
     if dw is not None or db is not None:
-        nbytes = nat.load().mednext_ln_bwd_workspace_size(outer, c, inner, code)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        nbytes = _workspace_size(outer, c, inner, code)
+        ws = stats.new_empty(nbytes // 4) if nbytes else None  # floats
     nat.launch("mednext_ln_bwd", x, dy.data_ptr(), x.data_ptr(), stats.data_ptr(), nat.ptr(weight), dx.data_ptr(),
                nat.ptr(dw), nat.ptr(db), nat.ptr(ws), nbytes, outer, c, inner, code, _param_code(x, weight, bias))
     return dx, dw, db

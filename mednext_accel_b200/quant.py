@@ -11,6 +11,8 @@ rounding to x's type.  Inference only: there is no gradient.
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 from torch import Tensor, nn
 from torch.library import custom_op
@@ -54,20 +56,26 @@ def quantize_int8(x: Tensor, dim: int = -1) -> tuple[Tensor, Tensor]:
     return q[:, :k], scale
 
 
+@lru_cache(maxsize=1024)
+def _workspace_size(outer: int, k: int, inner: int, n: int, code: int) -> int:
+    return nat.load().mednext_int8_linear_workspace_size(outer, k, inner, n, code)
+
+
 def _launch(x: Tensor, weight: Tensor, scale: Tensor, bias: Tensor | None, dim: int) -> Tensor:
     outer, k, inner = axis_sizes(x, dim)
     n, code = weight.shape[0], nat.dtype_code(x.dtype)
-    pitch = weight.stride(0)
-    if weight.stride(1) != 1 or pitch % 16 != 0 or pitch < k or weight.data_ptr() % 16 != 0:
+    pitch, at = weight.stride(0), weight.data_ptr()
+    if pitch % 16 or at % 16 or pitch < k or weight.stride(1) != 1:
         pitch = (k + 15) // 16 * 16
         held = weight.new_empty((n, pitch))
         held[:, :k] = weight
-        weight = held
-    y = torch.empty((*x.shape[:dim], n, *x.shape[dim + 1:]), dtype=x.dtype, device=x.device)
-    nbytes = nat.load().mednext_int8_linear_workspace_size(outer, k, inner, n, code)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    nat.launch("mednext_int8_linear", x, x.data_ptr(), weight.data_ptr(), scale.data_ptr(), nat.ptr(bias),
-               y.data_ptr(), nat.ptr(ws), nbytes, outer, k, inner, n, pitch, code)
+        weight, at = held, held.data_ptr()
+    y = x.new_empty((*x.shape[:dim], n, *x.shape[dim + 1:]))
+    nbytes = _workspace_size(outer, k, inner, n, code)
+    ws = weight.new_empty(nbytes) if nbytes else None  # bytes, like the weight
+    nat.launch("mednext_int8_linear", x, x.data_ptr(), at, scale.data_ptr(),
+               None if bias is None else bias.data_ptr(), y.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+               outer, k, inner, n, pitch, code)
     return y
 
 
