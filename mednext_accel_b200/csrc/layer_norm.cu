@@ -1108,10 +1108,16 @@ LnPlan plan_ln(const LnArgs& a, bool bwd) {
 }
 
 // Most weight-grad partials that a call makes: one per CTA of the backward kernel, four
-// CTAs per SM; at least four tokens each, so that the partials stay small beside the data.
-int dw_parts(long long tokens) { return (int)std::max(1LL, std::min((long long)kSms * 4, (tokens + 3) / 4)); }
+// CTAs per SM; at least four tokens each, so that the partials stay small beside the data, and
+// 64 MB of them or one per SM.  Rows past the register kernels: enough CTAs for the GPU over
+// the columns and the parts.
+int dw_parts(long long tokens, int C, long long inner) {
+  long long most = std::min(kSms * 4LL, std::max<long long>(kSms, (1LL << 23) / C));
+  if (inner == 1 && C > kRowThreads * 32) most = std::max(1LL, kSms * 8LL / ((C + 31) / 32));
+  return (int)std::max(1LL, std::min(most, (tokens + 3) / 4));
+}
 
-// Launches KERNEL<T, VEC, EPT, R> for a plan's vec and ept.
+// Launches the rows kernels for a plan's vec and ept.
 template <typename T, int VEC, int EPT, int R>
 int launch_rows(const LnArgs& a, const LnPlan& p, bool bwd, int parts, cudaStream_t s) {
   const size_t param = RowParam<T, VEC, EPT>::smem_bytes(p.G);
@@ -1202,15 +1208,14 @@ int ln_bwd(const LnArgs& a, void* dw, void* db, cudaStream_t s) {
   // one CTA per resident slot (the launch bounds leave 512 threads), one partial per CTA
   const int warps = p.form == kRows ? p.threads / 32 : std::max(1, p.S * p.P);
   const long long slots = (long long)kSms * std::max(1, 16 / warps);
-  int st, parts = (int)std::min<long long>(std::min<long long>(dw_parts(a.tokens), slots), std::max(1LL, p.units));
+  int st, parts = (int)std::min<long long>(std::min<long long>(dw_parts(a.tokens, a.C, a.inner), slots), std::max(1LL, p.units));
   if (p.form == kRows) {
     st = launch_rows_any_vec<T>(a, p, true, parts, s);
   } else if (p.form == kChan) {
     st = launch_chan_any_word<T>(a, p, true, parts, s);
   } else {
-    // enough CTAs for the GPU over the columns and the parts
     const long long cols = (a.C + 31) / 32;
-    parts = (int)std::min<long long>(dw_parts(a.tokens), std::max(1LL, (long long)kSms * 8 / cols));
+    parts = (int)std::min<long long>(dw_parts(a.tokens, a.C, 1), std::max(1LL, kSms * 8LL / cols));
     ln_rows_any_dx_kernel<T><<<(unsigned)std::min<long long>(a.tokens, kSms * 32), 256, 0, s>>>(a);
     st = record_launch();
     if (st != MEDNEXT_OK || a.part == nullptr) return st;
@@ -1267,7 +1272,7 @@ int mednext_ln_fwd(const void* x, const void* weight, const void* bias, void* y,
 
 size_t mednext_ln_bwd_workspace_size(int64_t outer, int64_t c, int64_t inner, int dtype) {
   if (ln_check(outer, c, inner, dtype, MEDNEXT_FLOAT32) != MEDNEXT_OK || outer * inner == 0) return 0;
-  return (size_t)dw_parts(outer * inner) * 2 * (size_t)c * sizeof(float);
+  return (size_t)dw_parts(outer * inner, (int)c, inner) * 2 * (size_t)c * sizeof(float);
 }
 
 int mednext_ln_bwd(const void* dy, const void* x, const float* stats, const void* weight, void* dx, void* dweight,
