@@ -356,8 +356,9 @@ int mednext_int8_quantize(const void* x, int8_t* q, float* scale, int64_t outer,
  * with q, scale of x as above; weight: 8-bit [n][weight_pitch], 16-byte aligned,
  * weight_pitch a multiple of 16 (columns past k are not used, but may be read up to a
  * multiple of 16); weight_scale [n], bias [n] or NULL (FLOAT32); y in x's type.  The
- * workspace is 16-byte aligned; its size is 0, and NULL is taken, for a few tokens.  The integer sum is exact, the rest fp32 with
- * one rounding.  No reference counterpart. */
+ * workspace is 16-byte aligned; its size is 0, and NULL is taken, for a few tokens and for
+ * a few hundred with a long k.  The integer sum is exact, the rest fp32 with one rounding.
+ * No reference counterpart. */
 size_t mednext_int8_linear_workspace_size(int64_t outer, int64_t k, int64_t inner, int64_t n,
                                           int dtype);
 int mednext_int8_linear(const void* x, const int8_t* weight, const float* weight_scale,

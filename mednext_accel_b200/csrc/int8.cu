@@ -339,6 +339,19 @@ __device__ __forceinline__ I8Tile i8_tile(const I8GemmArgs& p, int t) {
 // A staging buffer: an epilogue warp's 32 lanes, 128 bytes each (128-byte swizzle).
 constexpr int kI8StageBytes = 32 * 128;
 
+// Where a loop stands in a ring: counted, since a division by a runtime number of slots costs
+// more than the K block's products.
+struct RingAt {
+  int slot = 0;
+  uint32_t turn = 0;  // its lowest bit: the parity of the slot's current phase
+  __device__ __forceinline__ void next(int slots) {
+    if (++slot == slots) {
+      slot = 0;
+      ++turn;
+    }
+  }
+};
+
 struct I8Shared {
   uint64_t full[kI8MaxStages], empty[kI8MaxStages];
   uint64_t tfull[kI8MaxAcc], tempty[kI8MaxAcc];
@@ -479,13 +492,13 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   if (warp == 0) {
     if (lane == 0) {
       bool ok = true;
+      RingAt at;
       for (int i = 0; i < mine && ok; ++i) {
         int sample, a0, b0;
         decode(i, sample, a0, b0);
-        for (int kb = 0; kb < kblocks; ++kb) {
-          const int st = (int)(issued % p.stages);
-          const long long turn = issued / p.stages;
-          if (turn > 0 && !(ok = wait_or_abort(&sh.empty[st], (uint32_t)((turn - 1) & 1), abort))) break;
+        for (int kb = 0; kb < kblocks; ++kb, at.next(p.stages)) {
+          const int st = at.slot;
+          if (at.turn > 0 && !(ok = wait_or_abort(&sh.empty[st], (at.turn - 1) & 1, abort))) break;
           mbar_arrive_expect_tx(&sh.full[st], (uint32_t)(kI8BM * kI8BK + b_bytes));
           tma_load_3d(ringA + (size_t)st * (kI8BM * kI8BK), &mA, &sh.full[st], kb * kI8BK, a0, TOKENS_A ? sample : 0);
           tma_load_3d(ringB + (size_t)st * b_bytes, &mB, &sh.full[st], kb * kI8BK, b0, TOKENS_A ? 0 : sample);
@@ -496,16 +509,16 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   } else if (warp == 1) {
     if (lane == 0) {
       const uint32_t idesc = make_idesc_i8(kI8BM, p.bn);
-      long long q = 0;
+      RingAt at;
       bool ok = true;
       for (int i = 0; i < mine && ok; ++i) {
         const int acc = i % p.accs, turn = i / p.accs;
         if (turn > 0 && !wait_or_abort(&sh.tempty[acc], (uint32_t)((turn - 1) & 1), abort)) break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(acc * p.bn);
-        for (int kb = 0; kb < kblocks; ++kb, ++q) {
-          const int st = (int)(q % p.stages);
-          if (!(ok = wait_or_abort(&sh.full[st], (uint32_t)((q / p.stages) & 1), abort))) break;
+        for (int kb = 0; kb < kblocks; ++kb, at.next(p.stages)) {
+          const int st = at.slot;
+          if (!(ok = wait_or_abort(&sh.full[st], at.turn & 1, abort))) break;
           tc_fence_after();
           const uint32_t sa = smem_u32(ringA + (size_t)st * (kI8BM * kI8BK)), sb = smem_u32(ringB + (size_t)st * b_bytes);
           const int steps = min(kI8BK, p.K - kb * kI8BK + 31) / 32;  // 32 of K per instruction; zeros past K
@@ -698,13 +711,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
   if (warp == 0) {
     if (lane == 0) {
       bool ok = true;
+      RingAt at;
       for (int i = 0; i < mine && ok; ++i) {
         int sample, a0, b0;
         decode(i, sample, a0, b0);
-        for (int kb = 0; kb < kblocks; ++kb) {
-          const int st = (int)(issued % kI8PairStages);
-          const long long turn = issued / kI8PairStages;
-          if (turn > 0 && !(ok = wait_or_abort(&sh.empty[st], (uint32_t)((turn - 1) & 1), abort))) break;
+        for (int kb = 0; kb < kblocks; ++kb, at.next(kI8PairStages)) {
+          const int st = at.slot;
+          if (at.turn > 0 && !(ok = wait_or_abort(&sh.empty[st], (at.turn - 1) & 1, abort))) break;
           if (rank == 0) mbar_arrive_expect_tx(&sh.full[st], 4 * kHalf);  // both CTAs' bytes
           const uint32_t bar = cluster_addr(&sh.full[st], 0);
           tma_load_3d_pair(ringA + (size_t)st * kHalf, &mA, bar, kb * kI8BK, a0, TOKENS_A ? sample : 0);
@@ -716,16 +729,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = make_idesc_i8(2 * kI8BM, 256);
-      long long q = 0;
+      RingAt at;
       bool ok = true;
       for (int i = 0; i < mine && ok; ++i) {
         const int acc = i % kAccs, turn = i / kAccs;
         if (turn > 0 && !wait_or_abort(&sh.tempty[acc], (uint32_t)((turn - 1) & 1), abort)) break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(acc * 256);
-        for (int kb = 0; kb < kblocks; ++kb, ++q) {
-          const int st = (int)(q % kI8PairStages);
-          if (!(ok = wait_or_abort(&sh.full[st], (uint32_t)((q / kI8PairStages) & 1), abort))) break;
+        for (int kb = 0; kb < kblocks; ++kb, at.next(kI8PairStages)) {
+          const int st = at.slot;
+          if (!(ok = wait_or_abort(&sh.full[st], at.turn & 1, abort))) break;
           tc_fence_after();
           const uint32_t sa = smem_u32(ringA + (size_t)st * kHalf), sb = smem_u32(ringB + (size_t)st * kHalf);
           const int steps = min(kI8BK, p.K - kb * kI8BK + 31) / 32;
