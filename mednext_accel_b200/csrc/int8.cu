@@ -21,6 +21,7 @@ namespace {
 
 constexpr float kTinyMax = 127.f * 1.17549435e-38f;
 constexpr int kI8MaxK = 131072;
+constexpr int kI8MaxN = 1 << 22;
 constexpr int kI8Sms = 148;
 
 // The largest magnitude of a token as ordered bits: the bits of |x| as an unsigned
@@ -1144,6 +1145,465 @@ int launch_few(I8FewArgs a, cudaStream_t s) {
   return record_launch();
 }
 
+// ------------------------------ few hundred tokens: one cluster per tile ------------------------------
+// A few hundred tokens are too few 128-row tiles for the SMs, and a long K is a long chain of
+// loads in each of them: 2048 -> 512 channels at 8^3 are 32 CTAs of 16 K blocks, which an SM takes
+// in at about 60 GB/s.  Here a cluster of S CTAs takes 32 tokens and up to 256 output channels,
+// and its CTAs share K: each quantises its slice of the tokens into shared memory, as
+// operand B, and multiplies it with its slice of the weights (operand A, by TMA, under way while
+// x is read).  Two things cross the cluster, through distributed shared memory: a token's
+// maximum, and the integer sums, of which each CTA joins and stores 1 / S.  Maxima and integer
+// sums have no order, so the bits equal the other forms'.
+constexpr int kI8ClTokens = 32, kI8ClWorkers = 256, kI8ClPiece = 256;  // channels of a turn of the workers
+constexpr int kI8ClHeld = 2;  // turns whose values stay in registers: x is read once up to slices of 512 channels
+constexpr int kI8ClMt = 2, kI8ClSlice = 16, kI8ClStages = 8;
+constexpr int kI8ClRow = 36, kI8ClCol = 132;  // words between partial sums' rows: 16-byte rows without bank conflicts
+
+struct I8ClusterArgs {
+  const void* x;
+  const float* ws;
+  const float* bias;  // or NULL
+  void* y;
+  int inner, tokens;  // tokens of a sample
+  int tiles;          // tiles of a sample
+  int K, N;
+  int S, slice;       // CTAs of a cluster, 128-byte K blocks of a CTA
+  int mt, groups;     // tiles of 128 output channels per cluster, clusters per token tile
+  int stages;
+  int region;         // bytes of the weights' ring, later the partial sums
+  int vec_x, vec_y;   // 16-byte accesses
+};
+
+struct I8ClusterShared {
+  uint64_t full[kI8ClStages], empty[kI8ClStages];
+  uint64_t quantised, sums, drain;
+  uint32_t tmem_base;
+  int abort;
+  uint32_t most[kI8ClTokens];  // of this CTA's slice
+  float scale[kI8ClTokens];
+};
+
+__device__ __forceinline__ uint32_t peer_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ int4 peer_int4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// W tokens per lane (channels first: 1, or 2 neighbouring 16-bit ones), W = 0: rows.
+template <typename T, int W>
+__global__ void __launch_bounds__(kI8Threads, 1)
+    i8_cluster_kernel(const __grid_constant__ CUtensorMap mW, const __grid_constant__ I8ClusterArgs a) {
+  extern __shared__ uint8_t i8_raw[];
+  __shared__ I8ClusterShared sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(i8_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* qs = ring + a.region;  // [slice][32 tokens][128 bytes], 128-byte swizzle
+  int* part = reinterpret_cast<int*>(ring);
+
+  const int S = a.S, rank = (int)blockIdx.x % S, cluster = (int)blockIdx.x / S;
+  const int group = cluster % a.groups, tile = cluster / a.groups;
+  const int o = tile / a.tiles, v0 = (tile - o * a.tiles) * kI8ClTokens;  // sample and its first token
+  const int kblocks = (a.K + kI8BK - 1) / kI8BK, active = (kblocks + a.slice - 1) / a.slice;
+  const int kb0 = rank * a.slice, nkb = max(0, min(a.slice, kblocks - kb0));
+  const int n0 = group * a.mt * kI8BM, mt = min(a.mt, (a.N - n0 + kI8BM - 1) / kI8BM);
+  const uint32_t tmem_cols = (uint32_t)(32 * kI8ClMt);
+  const int blocks = nkb * mt;  // of weights
+
+  if (warp == 1) {
+    tmem_alloc(&sh.tmem_base, tmem_cols);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < a.stages; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
+    }
+    mbar_init(&sh.quantised, kI8ClWorkers);
+    mbar_init(&sh.sums, 1);
+    mbar_init(&sh.drain, 1);
+    sh.abort = 0;
+    fence_mbarrier_init();
+    tma_prefetch_map(&mW);
+  }
+  if (threadIdx.x < kI8ClTokens) sh.most[threadIdx.x] = 0;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem_base;
+  volatile int* abort = &sh.abort;
+  int issued = 0;
+  RingAt at{}, block{};  // block: tile of channels (slot) and K block (turn)
+  const auto issue = [&](int end) {  // weight blocks up to end
+    for (; issued < end; ++issued, at.next(a.stages), block.next(mt)) {
+      const int st = at.slot, kb = (int)block.turn, m = block.slot;
+      if (at.turn > 0 && !wait_or_abort(&sh.empty[st], (at.turn - 1) & 1, abort)) return;
+      mbar_arrive_expect_tx(&sh.full[st], (uint32_t)(kI8BM * kI8BK));
+      tma_load_3d(ring + (size_t)st * (kI8BM * kI8BK), &mW, &sh.full[st], (kb0 + kb) * kI8BK, n0 + m * kI8BM, 0);
+    }
+  };
+
+  if (warp == 0) {
+    if (lane == 0) issue(min(blocks, a.stages));
+    __syncwarp();
+    cluster_sync();  // the maxima
+    if (lane == 0) issue(blocks);
+  } else if (warp == 1) {
+    cluster_sync();
+    if (lane == 0 && nkb > 0 && wait_or_abort(&sh.quantised, 0, abort)) {
+      tc_fence_after();
+      constexpr uint32_t idesc = make_idesc_i8(kI8BM, kI8ClTokens);
+      bool ok = true;
+      for (int q = 0; q < blocks; ++q, at.next(a.stages), block.next(mt)) {
+        const int st = at.slot, kb = (int)block.turn, m = block.slot;
+        if (!(ok = wait_or_abort(&sh.full[st], at.turn & 1, abort))) break;
+        tc_fence_after();
+        const uint32_t sa = smem_u32(ring + (size_t)st * (kI8BM * kI8BK)), sb = smem_u32(qs + kb * (kI8ClTokens * kI8BK));
+        const int steps = min(kI8BK, a.K - (kb0 + kb) * kI8BK + 31) / 32;  // zeros past K
+        for (int ks = 0; ks < steps; ++ks)
+          mma_i8_ss(tmem + (uint32_t)(m * kI8ClTokens), make_sw128_desc(sa + ks * 32, 16, 1024),
+                    make_sw128_desc(sb + ks * 32, 16, 1024), idesc, kb > 0 || ks > 0 ? 1u : 0u);
+        mma_commit(&sh.empty[st]);
+      }
+      if (ok) mma_commit(&sh.sums);
+    }
+    __syncwarp();
+  } else {
+    const int wk = warp - 2;
+    const int k0 = kb0 * kI8BK, kq = k0 + nkb * kI8BK, kend = min(a.K, kq);  // quantised, and there to read
+    const int pieces = (nkb * kI8BK + kI8ClPiece - 1) / kI8ClPiece;
+    const T* x = static_cast<const T*>(a.x);
+    // 16 bytes of a token's row of operand B
+    const auto slot = [&](int token, int c) {
+      const int k = c - k0;
+      return qs + (k / kI8BK) * (kI8ClTokens * kI8BK) + token * kI8BK + (((k % kI8BK / 16) ^ (token & 7)) << 4);
+    };
+    if constexpr (W > 0) {
+      // lanes along the tokens, a warp has 32 channels of a piece
+      constexpr int TX = 32 / W, CH = 32 / W;
+      const int tx = lane % TX, cy = lane / TX, v = v0 + tx * W;
+      const bool in = v < a.inner;  // inner is even where W = 2
+      const T* px = x + (long long)o * a.K * a.inner + v;
+      uint32_t held[kI8ClHeld][CH];
+      const auto load = [&](uint32_t (&w)[CH], int piece) {
+#pragma unroll
+        for (int k = 0; k < CH; ++k) {
+          const int c = k0 + piece * kI8ClPiece + wk * 32 + cy * CH + k;
+          const bool ok = in && c < kend;
+          const T* p = px + (long long)c * a.inner;
+          if constexpr (W == 2) w[k] = ok ? *reinterpret_cast<const uint32_t*>(p) : 0u;
+          else if constexpr (sizeof(T) == 4) w[k] = ok ? __float_as_uint(*p) : 0u;
+          else w[k] = ok ? (uint32_t)*reinterpret_cast<const uint16_t*>(p) : 0u;
+        }
+      };
+      uint32_t m = 0;
+      for (int first = 0; first < pieces; first += kI8ClHeld) {
+#pragma unroll
+        for (int i = 0; i < kI8ClHeld; ++i) load(held[i], first + i);
+#pragma unroll
+        for (int i = 0; i < kI8ClHeld; ++i)
+#pragma unroll
+          for (int k = 0; k < CH; ++k) {
+            if constexpr (W == 2) m = __vmaxu2(m, held[i][k] & 0x7fff7fffu);
+            else m = max(m, held[i][k] & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fffu));
+          }
+      }
+      uint32_t most[W];
+      if constexpr (W == 2) {
+        m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, TX));
+        most[0] = Mag<T>::lo(m);
+        most[1] = Mag<T>::hi(m);
+      } else if constexpr (sizeof(T) == 4) {
+        most[0] = m;
+      } else {
+        most[0] = abs_bits(unpack2<T>(m).x);
+      }
+      if (cy == 0) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) atomicMax(&sh.most[tx * W + j], most[j]);
+      }
+      __syncwarp();
+      cluster_sync();
+#pragma unroll
+      for (int j = 0; j < W; ++j) most[j] = 0;
+      for (int r = 0; r < active; ++r) {
+        const uint32_t at = cluster_addr(&sh.most[tx * W], (uint32_t)r);
+#pragma unroll
+        for (int j = 0; j < W; ++j) most[j] = max(most[j], peer_u32(at + 4 * j));
+      }
+      TokenScale ts[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j) ts[j] = token_scale(most[j]);
+      if (wk == 0 && cy == 0) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) sh.scale[tx * W + j] = ts[j].scale;
+      }
+      for (int first = 0; first < pieces; first += kI8ClHeld) {
+        if (pieces > kI8ClHeld) {
+#pragma unroll
+          for (int i = 0; i < kI8ClHeld; ++i) load(held[i], first + i);
+        }
+#pragma unroll
+        for (int i = 0; i < kI8ClHeld; ++i)
+#pragma unroll
+          for (int h = 0; h < CH / 16; ++h) {
+            const int c = k0 + (first + i) * kI8ClPiece + wk * 32 + cy * CH + h * 16;
+            if (c >= kq) break;
+            uint32_t b[W][4];
+            quantize16<T, W>(held[i] + h * 16, ts, b);
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+              const uint32_t keep = most[j] >= 0x7f800000u ? 0u : 0xffffffffu;
+              *reinterpret_cast<uint4*>(slot(tx * W + j, c)) =
+                  make_uint4(b[j][0] & keep, b[j][1] & keep, b[j][2] & keep, b[j][3] & keep);
+            }
+          }
+      }
+    } else {
+      // a warp has four tokens, a lane 8 neighbouring values of each
+      using M = Mag<T>;
+      using Words = typename M::Word[4][4];
+      Words held[kI8ClHeld];
+      const auto load = [&](Words& w, int piece) {
+        const int c = k0 + piece * kI8ClPiece + lane * 8;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int token = v0 + wk * 4 + t;
+          const T* p = x + (long long)token * a.K + c;
+          if (a.vec_x) {  // K is a multiple of the vector's values
+            constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll
+            for (int h = 0; h < 8 / E; ++h) {
+              const uint4 r = token < a.tokens && c + h * E < kend ? *reinterpret_cast<const uint4*>(p + h * E)
+                                                                   : make_uint4(0, 0, 0, 0);
+              memcpy(&w[t][h * E / 2], &r, 16);
+            }
+          } else {
+            T e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = token < a.tokens && c + i < kend ? p[i] : from_acc<T>(0.f);
+            memcpy(w[t], e, sizeof(e));
+          }
+        }
+      };
+      typename M::Max m[4] = {};
+      for (int first = 0; first < pieces; first += kI8ClHeld) {
+#pragma unroll
+        for (int p = 0; p < kI8ClHeld; ++p) load(held[p], first + p);
+#pragma unroll
+        for (int p = 0; p < kI8ClHeld; ++p)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m[t] = M::join(m[t], held[p][t][i]);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint32_t most = __reduce_max_sync(0xffffffffu, max(M::lo(m[t]), M::hi(m[t])));
+        if (lane == 0) sh.most[wk * 4 + t] = most;
+      }
+      __syncwarp();
+      cluster_sync();
+      uint32_t most[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        most[t] = lane < active ? peer_u32(cluster_addr(&sh.most[wk * 4 + t], (uint32_t)lane)) : 0u;
+      TokenScale ts[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        most[t] = __reduce_max_sync(0xffffffffu, most[t]);
+        ts[t] = token_scale(most[t]);
+        if (lane == 0) sh.scale[wk * 4 + t] = ts[t].scale;
+      }
+      for (int first = 0; first < pieces; first += kI8ClHeld) {
+        if (pieces > kI8ClHeld) {
+#pragma unroll
+          for (int p = 0; p < kI8ClHeld; ++p) load(held[p], first + p);
+        }
+#pragma unroll
+        for (int p = 0; p < kI8ClHeld; ++p) {
+          const int c = k0 + (first + p) * kI8ClPiece + lane * 8;
+          if (c >= kq) break;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const uint32_t keep = most[t] >= 0x7f800000u ? 0u : 0xffffffffu;
+            uint32_t b[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 f = scaled2(M::value(held[p][t][2 * i]), ts[t].inverse, ts[t].inverse),
+                           g = scaled2(M::value(held[p][t][2 * i + 1]), ts[t].inverse, ts[t].inverse);
+              b[i] = low_bytes(f.x, f.y, g.x, g.y) & keep;
+            }
+            *reinterpret_cast<uint2*>(slot(wk * 4 + t, c) + (c & 8)) = make_uint2(b[0], b[1]);
+          }
+        }
+      }
+      __syncwarp();
+    }
+    fence_async_smem();
+    mbar_arrive(&sh.quantised);
+    // the partial sums take the place of the weights, which the products have read
+    if (nkb > 0 && __all_sync(0xffffffffu, wait_or_abort(&sh.sums, 0, abort))) {
+      tc_fence_after();
+      const int q4 = warp & 3;
+      const int m = wk >> 2;  // a warpgroup per tile of channels
+      if (m < mt) {
+        uint32_t r[32];
+        tmem_ld32(tmem + (uint32_t)(m * kI8ClTokens) + ((uint32_t)(q4 * 32) << 16), r);
+        tmem_ld_wait();
+        if constexpr (W > 0) {  // [channel][token]
+          int* at = part + (m * kI8BM + q4 * 32 + lane) * kI8ClRow;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4*>(at + 4 * i) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+        } else {  // [tile][token][channel]
+          int* at = part + m * (kI8ClTokens * kI8ClCol) + q4 * 32 + lane;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) at[i * kI8ClCol] = (int)r[i];
+        }
+      }
+      tc_fence_before();
+    }
+    __syncwarp();
+  }
+  // Eight outputs along y's rows per worker: 1 / S of the cluster's.
+  const int rows = mt * kI8BM / S, per = W > 0 ? kI8ClTokens / 8 : rows / 8;
+  const int hi = ((int)threadIdx.x - 64) / per, lo = ((int)threadIdx.x - 64) - hi * per;
+  const int row = rank * rows + (W > 0 ? hi : lo * 8), token = W > 0 ? lo * 8 : hi;  // of the cluster's
+  const int n = n0 + row, v = v0 + token;
+  const bool mine = warp >= 2 && (W > 0 ? hi < rows : hi < kI8ClTokens) && n < a.N && v < a.tokens;
+  constexpr int kChans = W > 0 ? 1 : 8;
+  float ws[kChans], bias[kChans];
+#pragma unroll
+  for (int e = 0; e < kChans; ++e) {
+    ws[e] = mine && n + e < a.N ? a.ws[n + e] : 0.f;
+    bias[e] = mine && n + e < a.N && a.bias != nullptr ? a.bias[n + e] : 0.f;
+  }
+  __syncwarp();
+  cluster_sync();  // every CTA's partial sums
+  if (mine) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const int* at = part + (W > 0 ? row * kI8ClRow + token
+                                  : row / kI8BM * (kI8ClTokens * kI8ClCol) + token * kI8ClCol + row % kI8BM);
+    int4 r[8][2];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      r[s][0] = r[s][1] = make_int4(0, 0, 0, 0);
+      if (s >= active) continue;
+      const uint32_t peer = cluster_addr(at, (uint32_t)s);
+      r[s][0] = peer_int4(peer);
+      r[s][1] = peer_int4(peer + 16);
+    }
+    int sum[8] = {};
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        sum[4 * h] += r[s][h].x;
+        sum[4 * h + 1] += r[s][h].y;
+        sum[4 * h + 2] += r[s][h].z;
+        sum[4 * h + 3] += r[s][h].w;
+      }
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = W > 0 ? 0 : e;
+      f[e] = fmaf((float)sum[e] * sh.scale[W > 0 ? token + e : token], ws[c], bias[c]);
+    }
+    const int left = W > 0 ? a.tokens - v : a.N - n;  // of y's row
+    T* out = static_cast<T*>(a.y) + (W > 0 ? ((long long)o * a.N + n) * a.inner + v : (long long)v * a.N + n);
+#pragma unroll
+    for (int h = 0; h < 8 / E; ++h) {
+      if (a.vec_y) {  // y's rows are whole vectors
+        if (h * E < left) *reinterpret_cast<uint4*>(out + h * E) = pack16<T>(f + h * E);
+      } else {
+#pragma unroll
+        for (int e = h * E; e < (h + 1) * E; ++e)
+          if (e < left) out[e] = from_acc<T>(f[e]);
+      }
+    }
+  }
+  __syncwarp();
+  if (*abort && lane == 0) {
+    if (warp == 0) drain_ring(sh.full, a.stages, issued);
+    if (warp == 1) drain_mma(&sh.drain);
+  }
+  __syncwarp();
+  cluster_sync();  // no CTA's memory is in use by the others any more
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_cols);
+  }
+}
+
+// Whether the clusters take a product, and how: where K is long and all of them are resident at
+// once (the occupancy query gives 15 clusters of 8, 33 of 4).  Tokens x K -> N in bf16, us,
+// against the two kernels: channels first 512 x 2048 -> 512 13.9, 15.3; 512 x 1024 -> 256
+// 9.0, 10.0; 64 x 2048 -> 512 8.7, 14.6; rows 16 x 4096 -> 1024 10.1, 18.4, 64 x 4096 -> 1024 13.7, 18.6.
+// In two waves 216 x 2048 -> 2048 took 17.9, 15.4, and with a shorter K, rows 16 x 1024 -> 4096 9.0,
+// 8.2, channels first 64 x 512 -> 512 7.4, 7.2 (rows are quantised faster).
+bool cluster_takes(long long outer, int K, long long inner, int N, I8ClusterArgs* a) {
+  const long long tokens = inner > 1 ? inner : outer, samples = inner > 1 ? outer : 1;
+  const int kblocks = (K + kI8BK - 1) / kI8BK, mtiles = (N + kI8BM - 1) / kI8BM;
+  if (kblocks < (inner > 1 ? 7 : 16) || tokens > 4096 || samples > 128) return false;
+  a->tiles = (int)((tokens + kI8ClTokens - 1) / kI8ClTokens);
+  const auto fits = [&](int S, int mt, int ctas) {
+    a->S = S;
+    a->mt = mt;
+    a->slice = (kblocks + S - 1) / S;
+    a->groups = (mtiles + mt - 1) / mt;
+    return a->slice <= kI8ClSlice && samples * a->tiles * a->groups * S <= ctas;
+  };
+  return (kblocks >= 16 && fits(8, 1, 112)) || fits(4, 1, 128) || (kblocks >= 16 && mtiles > 1 && fits(4, 2, 128));
+}
+
+template <typename T>
+int launch_cluster(I8ClusterArgs a, const int8_t* w, long long w_pitch, long long outer, cudaStream_t s) {
+  a.tokens = a.inner > 1 ? a.inner : (int)outer;
+  const bool chan = a.inner > 1, pair = sizeof(T) == 2 && a.inner % 2 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 3) == 0;
+  constexpr int E = 16 / (int)sizeof(T);
+  a.vec_x = a.K % E == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+  a.vec_y = (chan ? a.inner : a.N) % E == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
+  a.stages = std::min(kI8ClStages, a.mt * a.slice);
+  const int sums = a.mt * (chan ? kI8BM * kI8ClRow : kI8ClTokens * kI8ClCol) * (int)sizeof(int);
+  a.region = (std::max(a.stages * kI8BM * kI8BK, sums) + 1023) / 1024 * 1024;
+  const size_t smem = (size_t)a.region + (size_t)a.slice * (kI8ClTokens * kI8BK) + 1024;
+  CUtensorMap mW;
+  if (!tma::encode_rows_8bit(&mW, w, a.K, a.N, 1, w_pitch, kI8BM)) {
+    note_cuda_error(cudaErrorInvalidValue);
+    return MEDNEXT_ERR_CUDA;
+  }
+  const auto run = [&](auto kern) {
+    const int st = ensure_smem(kern, smem);
+    if (st != MEDNEXT_OK) return st;
+    const long long samples = chan ? outer : 1;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)a.S;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(samples * a.tiles * a.groups * a.S));
+    cfg.blockDim = dim3(kI8Threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kern, mW, a);
+    return record_launch();
+  };
+  if (!chan) return run(i8_cluster_kernel<T, 0>);
+  if constexpr (sizeof(T) == 2)
+    if (pair) return run(i8_cluster_kernel<T, 2>);
+  return run(i8_cluster_kernel<T, 1>);
+}
+
 int num_sms() {
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
@@ -1314,6 +1774,12 @@ int launch_linear(const void* x, const int8_t* w, const float* ws, long long w_p
     a.outer = (int)outer; a.inner = (int)inner; a.K = K; a.N = N;
     return launch_narrow<T>(a, s);
   }
+  I8ClusterArgs c{};
+  if (cluster_takes(outer, K, inner, N, &c)) {
+    c.x = x; c.ws = ws; c.bias = bias; c.y = y;
+    c.inner = (int)inner; c.K = K; c.N = N;
+    return launch_cluster<T>(c, w, w_pitch, outer, s);
+  }
   int st = launch_quantize<T>(x, q, qs, outer, K, inner, pitch16(K), s);
   if (st != MEDNEXT_OK) return st;
   return launch_gemm<T>(q, qs, pitch16(K), w, ws, w_pitch, bias, y, outer, inner, K, N, s);
@@ -1352,9 +1818,12 @@ int mednext_int8_quantize(const void* x, int8_t* q, float* scale, int64_t outer,
   }
 }
 
-// The workspace holds the tokens' 8-bit rows, then their scales; a few tokens need none.
+// The workspace holds the tokens' 8-bit rows, then their scales; the forms that quantise into
+// shared memory for any alignment need none.
 size_t mednext_int8_linear_workspace_size(int64_t outer, int64_t k, int64_t inner, int64_t n, int dtype) {
-  if (i8_check(outer, k, inner, dtype) != MEDNEXT_OK || n <= 0 || few_takes(outer * inner, (int)k)) return 0;
+  if (i8_check(outer, k, inner, dtype) != MEDNEXT_OK || n <= 0 || n > kI8MaxN) return 0;
+  I8ClusterArgs c{};
+  if (few_takes(outer * inner, (int)k) || cluster_takes(outer, (int)k, inner, (int)n, &c)) return 0;
   const size_t tokens = (size_t)(outer * inner);
   return tokens * (size_t)pitch16(k) + (tokens * sizeof(float) + 15) / 16 * 16;
 }
@@ -1364,7 +1833,7 @@ int mednext_int8_linear(const void* x, const int8_t* weight, const float* weight
                         int64_t weight_pitch, int dtype, mednext_stream_t stream) {
   const int st = i8_check(outer, k, inner, dtype);
   if (st != MEDNEXT_OK) return st;
-  if (n <= 0 || n > ((int64_t)1 << 22) || weight_pitch < k || weight_pitch % 16 != 0 ||
+  if (n <= 0 || n > kI8MaxN || weight_pitch < k || weight_pitch % 16 != 0 ||
       weight_pitch > ((int64_t)1 << 30))
     return MEDNEXT_ERR_BAD_SHAPE;
   if (outer * inner == 0) return MEDNEXT_OK;

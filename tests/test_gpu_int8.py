@@ -267,3 +267,80 @@ def test_large_rows(t, k, n, dtype):
 def test_large_channels_first(outer, k, v, n):
     w, s, b = weights(n, k, seed=v)
     check(activations((outer, k, v), torch.bfloat16, seed=n), w, s, b, 1)
+
+
+# A few hundred tokens and a long K share K over a cluster of SMs: whole and ragged slices, SMs
+# without a slice, K past what a slice's registers hold, ragged tiles of tokens and channels.
+CLUSTERED = [(9, 769, 1), (31, 896, 128), (33, 1024, 5), (100, 1921, 130), (64, 2048, 512), (512, 2048, 512), (17, 2049, 257),
+             (70, 2500, 384), (64, 4096, 1024), (200, 4100, 100), (16, 8200, 127), (40, 16384, 136), (24, 16400, 64),
+             (130, 2031, 77), (32, 2176, 129)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("t,k,n", CLUSTERED)
+def test_long_rows(t, k, n, dtype):
+    w, s, b = weights(n, k, seed=t)
+    check(activations((t, k), dtype, seed=k), w, s, b, -1)
+    check(activations((t, k), dtype, seed=k), w, s, None, -1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("outer,k,v,n", [
+    (1, 2048, 512, 512), (1, 1024, 343, 256), (2, 1000, 64, 300), (3, 2048, 27, 130), (1, 4096, 125, 64), (1, 900, 10, 1),
+    (4, 1025, 33, 129), (1, 16384, 34, 40), (1, 2300, 216, 512), (7, 1024, 30, 128), (1, 8192, 9, 257), (1, 769, 32, 128),
+])
+def test_deep_volumes(outer, k, v, n, dtype):
+    w, s, b = weights(n, k, seed=v)
+    check(activations((outer, k, v), dtype, seed=n), w, s, b, 1)
+    check(activations((outer, k, v), dtype, seed=n), w, s, None, 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_long_tokens_off_their_alignment(dtype):
+    """x at any element, in rows and channels first: the bits of an aligned copy."""
+    w, s, b = weights(200, 2048, seed=3)
+    for shape, dim in (((65, 2048), 1), ((2, 2048, 30), 1)):
+        x = activations(shape, dtype, seed=4)
+        held = torch.empty(x.numel() + 3, dtype=dtype, device="cuda")
+        moved = held[3:].view(shape)
+        moved.copy_(x)
+        assert moved.data_ptr() % 16 and torch.equal(mx.int8_linear(moved, w, s, b, dim=dim), mx.int8_linear(x, w, s, b, dim=dim))
+    assert nat.device_error() == 0
+
+
+def test_long_tokens_that_are_zero_or_not_finite():
+    w, s, b = weights(150, 2048, seed=5)
+    for shape, dim in (((40, 2048), 1), ((1, 2048, 40), 1)):
+        x = activations(shape, torch.bfloat16, seed=6)
+        tokens = x if shape[0] == 40 else x[0].t()  # views
+        tokens[3] = 0
+        tokens[11, 2047] = float("inf")
+        tokens[20, 0] = float("nan")
+        tokens[39, 700] = -float("inf")
+        y = mx.int8_linear(x, w, s, b, dim=dim)
+        rows = y if shape[0] == 40 else y[0].t()
+        bad = torch.tensor([11, 20, 39], device="cuda")
+        good = torch.ones(40, dtype=torch.bool, device="cuda")
+        good[bad] = False
+        assert rows[bad].isnan().all() and rows[good].isfinite().all()
+        assert torch.equal(rows[3], b.to(torch.bfloat16))
+    assert nat.device_error() == 0
+
+
+def test_long_tokens_are_the_same_bits_in_any_company():
+    """A token's result does not depend on the other tokens of the call: integer sums have no order, and
+    the forms for few, some and many tokens round alike."""
+    w, s, b = weights(300, 2048, seed=7)
+    x = activations((5000, 2048), torch.bfloat16, seed=8)
+    y = mx.int8_linear(x, w, s, b)
+    for start, count in ((0, 5), (5, 64), (69, 300), (4000, 33)):
+        assert torch.equal(mx.int8_linear(x[start:start + count], w, s, b), y[start:start + count])
+    v = x[:300].t().contiguous()[None]
+    assert torch.equal(mx.int8_linear(v, w, s, b, dim=1)[0].t(), y[:300])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        again = [mx.int8_linear(x[:64], w, s, b) for _ in range(20)]
+    stream.synchronize()
+    assert all(torch.equal(a, y[:64]) for a in again)
+    assert nat.device_error() == 0
