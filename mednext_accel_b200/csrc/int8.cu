@@ -32,12 +32,12 @@ struct TokenScale {
   float scale;    // s_t
   float inverse;  // 127 / m_t, 0 where m_t is not finite
 };
+__device__ __forceinline__ float token_inverse(uint32_t max_bits) {
+  return max_bits >= 0x7f800000u ? 0.f : __fdiv_rn(127.f, fmaxf(__uint_as_float(max_bits), kTinyMax));
+}
 __device__ __forceinline__ TokenScale token_scale(uint32_t max_bits) {
-  TokenScale s;
   const float m = max_bits >= 0x7f800000u ? __uint_as_float(max_bits) : fmaxf(__uint_as_float(max_bits), kTinyMax);
-  s.scale = __fdiv_rn(m, 127.f);
-  s.inverse = max_bits >= 0x7f800000u ? 0.f : __fdiv_rn(127.f, m);
-  return s;
+  return {__fdiv_rn(m, 127.f), token_inverse(max_bits)};
 }
 // ------------------------------ quantisation ------------------------------
 // rint(v * inverse) as the low byte of the sum with 1.5 * 2^23 (the sum's unit is 1, so its
@@ -322,6 +322,7 @@ struct I8GemmArgs {
   int N;                  // output channels
   int bn, stages, accs;
   int share;  // the two groups share each tile
+  int groups, copies;  // of quantising warps, of the channels in operand A (the medium form)
   int a_tiles, b_tiles, samples;  // tiles of one sample
 };
 
@@ -1035,8 +1036,7 @@ size_t narrow_smem(int K, int N, int W, int P) {
   return (size_t)narrow_weight_bytes(K, N) + (size_t)P * (narrow_tile_bytes(K, W) + S * mt_store * kNarrowStage) + 1024;
 }
 // Whether the one-kernel form takes a product: K and N small enough that bytes are its bound
-// (bf16, 64^3 voxels: 64 -> 192 channels 48 us against 51 us in two kernels, but 192 -> 64
-// 65 us against 64, 128 -> 512 34 against 22), whole 16-byte rows, and enough tiles.
+// (bf16, 64^3 voxels: 64 -> 192 channels 42 us against 51 us in two kernels; wider ones go to the medium form), whole 16-byte rows, and enough tiles.
 bool narrow_takes(const void* x, const void* y, long long outer, int K, long long inner, int N, size_t esz) {
   return K <= 64 && N <= 256 && inner % (16 / (long long)esz) == 0 && reinterpret_cast<uintptr_t>(x) % 4 == 0 &&
          reinterpret_cast<uintptr_t>(y) % 16 == 0 && outer * ((inner + 63) / 64) >= 2 * kI8Sms;
@@ -1623,6 +1623,352 @@ bool i8_maps(const I8GemmArgs& p, bool tokens_a, bool staged, const int8_t* a, l
                                      CU_TENSOR_MAP_SWIZZLE_128B));
 }
 
+// ------------------------------ medium K in one kernel, channels first ------------------------------
+// Between the narrow form and the large one (K up to 256, N up to 512), the 8-bit rows' way through
+// memory is a third or more of the bytes, and two kernels are two ramps.  Here persistent CTAs keep
+// the weights in shared memory (operand A) and take 256 bytes of each channel per tile (128 tokens
+// of 16-bit data, 64 of fp32): one warp per 32 channels loads them into registers and quantises them into
+// operand B; the product (tcgen05 kind::i8) goes into one of one to four accumulators, and other warps
+// scale it and store it by TMA.
+//
+// The rows' length is what counts: read in 128-byte pieces of 256 channels, HBM gives 4.6 TB/s here,
+// in 256-byte pieces 6.3.  (With 128-byte pieces, by TMA or by 16-byte asynchronous copies into a ring,
+// 128 -> 32 channels at 64^3 took 33 us.)  A lane holds W neighbouring tokens; token W l + j is operand
+// B's row 32 j + l, so that eight lanes' 16-byte stores meet different banks, and the accumulator's
+// columns 32 j + l come together again in the registers of the thread that stores them.
+//
+// bf16, 64^3 voxels, against the two kernels: 128 -> 32 28.7 us, 42.5; 192 -> 64 40, 63; 128 -> 128 36, 48;
+// 128 -> 512 93, 113; at 128^3 128 -> 32 150, 298 (4.5 TB/s); at 24^3 192 -> 64 7.9, 9.9.  What bounds it now is the
+// turn of a group of quantising warps (its loads' latency and about 700 instructions).
+constexpr int kI8MidK = 256;
+constexpr int kI8MidWarps = 12, kI8MidGroups = 4;  // at most
+constexpr int kI8MidScales = kI8MidGroups + kI8MaxAcc;
+
+struct I8MidShared {
+  uint64_t qfull[kI8MidGroups], qempty[kI8MidGroups];  // operand B
+  uint64_t tfull[kI8MaxAcc], tempty[kI8MaxAcc];
+  uint64_t weights, drain;
+  uint32_t tmem_base;
+  int abort;
+  // Scales of the last tiles' tokens.  A tile's are written once the last product of its operand B is
+  // done, which began after its accumulator's last tile was stored: as many as both have are enough.
+  alignas(16) float scale[kI8MidScales][128];
+  alignas(16) uint2 most[2][kI8MidWarps][32];  // by a warp's channels
+};
+
+// Whether one of the warps' threads failed: the same answer for all of a barrier's n threads.
+__device__ __forceinline__ bool any_at_barrier(int id, int n, bool failed) {
+  int any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.s32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.s32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(id), "r"(n), "r"((int)failed)
+      : "memory");
+  return any != 0;
+}
+
+// p: a_* the output channels, b_* the tokens; a_tiles and b_tiles count tiles of 128 channels and of
+// bn tokens.  WARPS quantise, EPI scale and store.
+template <typename T, int WARPS, int EPI>
+__global__ void __launch_bounds__(32 * (2 + EPI + WARPS), 1)
+    i8_mid_kernel(const T* __restrict__ x_all, const __grid_constant__ CUtensorMap mW,
+                  const __grid_constant__ CUtensorMap mY, const __grid_constant__ I8GemmArgs p) {
+  constexpr int W = 8 / (int)sizeof(T), TOK = 32 * W;  // tokens of a lane, of a tile
+  extern __shared__ uint8_t i8_raw[];
+  __shared__ I8MidShared sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kblocks = (p.K + kI8BK - 1) / kI8BK, mt = p.a_tiles, S = (p.K + 31) / 32;
+  const int groups = p.groups, buffers = max(2, groups);  // of quantising warps, tiles in turn; of operand B
+  const int q_bytes = kblocks * TOK * kI8BK;
+  uint8_t* wsm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(i8_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* qsm = wsm + mt * kblocks * (kI8BM * kI8BK);
+  uint8_t* stage = qsm + buffers * q_bytes;
+  uint32_t tmem_cols = 32;
+  while (tmem_cols < (uint32_t)(p.accs * mt * TOK)) tmem_cols *= 2;
+
+  if (warp == 1) {
+    tmem_alloc(&sh.tmem_base, tmem_cols);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < buffers; ++i) {
+      mbar_init(&sh.qfull[i], 32 * S);
+      mbar_init(&sh.qempty[i], 1);
+    }
+    for (int i = 0; i < p.accs; ++i) {
+      mbar_init(&sh.tfull[i], 1);
+      mbar_init(&sh.tempty[i], 32 * EPI);
+    }
+    mbar_init(&sh.weights, 1);
+    mbar_init(&sh.drain, 1);
+    sh.abort = 0;
+    fence_mbarrier_init();
+    tma_prefetch_map(&mW);
+    tma_prefetch_map(&mY);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem_base;
+  volatile int* abort = &sh.abort;
+  const int tiles = p.b_tiles * p.samples;
+  const int mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+  const auto decode = [&](int i, int& sample, int& v0) {
+    const int t = (int)blockIdx.x + i * (int)gridDim.x;
+    sample = t / p.b_tiles;
+    v0 = (t - sample * p.b_tiles) * TOK;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&sh.weights, (uint32_t)(mt * kblocks * (kI8BM * kI8BK)));
+      for (int kb = 0; kb < kblocks; ++kb)
+        for (int m = 0; m < mt; ++m)
+          for (int r = 0; r < p.copies; ++r)
+            tma_load_3d(wsm + (kb * mt + m) * (kI8BM * kI8BK) + r * (kI8BM / p.copies * kI8BK), &mW, &sh.weights, kb * kI8BK,
+                        m * kI8BM, 0);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && wait_or_abort(&sh.weights, 0, abort)) {
+      const uint32_t idesc = make_idesc_i8(kI8BM, TOK);
+      RingAt q, acc;
+      for (int i = 0; i < mine; ++i, q.next(buffers), acc.next(p.accs)) {
+        if (acc.turn > 0 && !wait_or_abort(&sh.tempty[acc.slot], (acc.turn - 1) & 1, abort)) break;
+        if (!wait_or_abort(&sh.qfull[q.slot], q.turn & 1, abort)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(acc.slot * mt * TOK);
+        for (int kb = 0; kb < kblocks; ++kb) {
+          const uint32_t sb = smem_u32(qsm + q.slot * q_bytes + kb * (TOK * kI8BK));
+          const int steps = min(kI8BK, p.K - kb * kI8BK + 31) / 32;  // zeros past K
+          for (int m = 0; m < mt; ++m) {
+            const uint32_t sa = smem_u32(wsm + (kb * mt + m) * (kI8BM * kI8BK));
+            for (int ks = 0; ks < steps; ++ks)
+              mma_i8_ss(d + (uint32_t)(m * TOK), make_sw128_desc(sa + ks * 32, 16, 1024),
+                        make_sw128_desc(sb + ks * 32, 16, 1024), idesc, kb > 0 || ks > 0 ? 1u : 0u);
+          }
+        }
+        mma_commit(&sh.qempty[q.slot]);
+        mma_commit(&sh.tfull[acc.slot]);
+      }
+    }
+  } else if (warp < 2 + EPI) {
+    // Pieces of 32 channels x 128 bytes of tokens, in turn among the groups of four warps.  A warp reads
+    // 32 of the accumulator's 128 lanes: with 64 channels or fewer they are there twice, with 32 four
+    // times, and the copies' warps take pieces in turn too.
+    constexpr int E = 16 / (int)sizeof(T);
+    const int e = warp - 2, q4 = warp & 3, q_chan = q4 % (4 / p.copies);
+    const int sharers = EPI / 4 * p.copies, me = (e >> 2) * p.copies + q4 / (4 / p.copies);
+    int turn = 0;  // of the next tile's first piece
+    uint8_t* stg = stage + e * kI8StageBytes;
+    RingAt acc;
+    for (int i = 0; i < mine; ++i, acc.next(p.accs)) {
+      int sample, v0;
+      decode(i, sample, v0);
+      if (!__all_sync(0xffffffffu, wait_or_abort(&sh.tfull[acc.slot], acc.turn & 1, abort))) break;
+      tc_fence_after();
+      const float* scales = sh.scale[i % kI8MidScales];
+      for (int piece = 0; piece < 2 * mt; ++piece) {
+        const bool my_turn = turn == me;
+        if (++turn == sharers) turn = 0;
+        const int m = piece >> 1, c = piece & 1, r0 = m * kI8BM + q_chan * 32, n = r0 + lane;
+        if (!my_turn || r0 >= p.a_rows) continue;
+        if (v0 + c * (16 * W) >= p.b_rows) continue;
+        uint32_t r[W][16];
+        const uint32_t at = tmem + (uint32_t)((acc.slot * mt + m) * TOK + 16 * c) + ((uint32_t)(q4 * 32) << 16);
+#pragma unroll
+        for (int j = 0; j < W; ++j) tmem_ld16(at + 32 * j, r[j]);
+        const float ws = n < p.a_rows ? p.a_scale[n] : 0.f, bias = n < p.a_rows && p.bias != nullptr ? p.bias[n] : 0.f;
+        if (lane == 0) bulk_wait_read<0>();  // the last store has read the buffer
+        __syncwarp();
+        tmem_ld_wait();
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {  // 16 bytes of tokens
+          float f[E];
+#pragma unroll
+          for (int h = 0; h < E; h += 4) {
+            const float4 ts = *reinterpret_cast<const float4*>(scales + c * (16 * W) + u * E + h);
+            const float tv[4] = {ts.x, ts.y, ts.z, ts.w};
+#pragma unroll
+            for (int k = 0; k < 4; k += 2) {
+              const int t = u * E + h + k;  // token of the piece: W i + j
+              const float2 v = make_float2((float)(int)r[t % W][t / W], (float)(int)r[(t + 1) % W][(t + 1) / W]);
+              const float2 o = __ffma2_rn(__fmul2_rn(v, make_float2(tv[k], tv[k + 1])), make_float2(ws, ws),
+                                          make_float2(bias, bias));
+              f[h + k] = o.x;
+              f[h + k + 1] = o.y;
+            }
+          }
+          *reinterpret_cast<uint4*>(stg + lane * 128 + ((u ^ (lane & 7)) << 4)) = pack16<T>(f);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d(&mY, stg, v0 + c * (16 * W), r0, sample);
+          bulk_commit();
+        }
+      }
+      __syncwarp();
+      tc_fence_before();
+      mbar_arrive(&sh.tempty[acc.slot]);
+    }
+    if (lane == 0) bulk_wait_all();
+  } else {
+    const int u = warp - 2 - EPI, group = u / S, s = u - group * S;
+    if (group < groups) {
+      const int rows = min(32, p.K - s * 32);  // channels of this warp
+      uint32_t xa[32], xb[32];
+      const auto load = [&](int i) {
+        int sample, v0;
+        decode(i, sample, v0);
+        const int v = v0 + lane * W;
+        const bool in = i < mine && v < p.b_rows;  // b_rows is a multiple of W
+        const T* px = x_all + ((long long)sample * p.K + s * 32) * p.b_rows + v;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          const uint2 w = in && k < rows ? *reinterpret_cast<const uint2*>(px) : make_uint2(0u, 0u);
+          xa[k] = w.x;
+          xb[k] = w.y;
+          px += p.b_rows;
+          asm volatile("" : "+l"(px));  // one address in flight, not 32
+        }
+      };
+      load(group);
+      bool failed = false;
+      for (int i = group, turn = 0; i < mine; i += groups, ++turn) {
+        uint2 m = make_uint2(0u, 0u);
+        const auto join = [](uint32_t a, uint32_t b) { return sizeof(T) == 2 ? __vmaxu2(a, b) : max(a, b); };
+        constexpr uint32_t kMag = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) m = make_uint2(join(m.x, xa[k] & kMag), join(m.y, xb[k] & kMag));
+        uint2(*maxima)[32] = sh.most[turn & 1] + group * S;
+        maxima[s][lane] = m;
+        // a warp that gave up says so here: the group leaves together
+        if (any_at_barrier(1 + group, 32 * S, failed)) break;
+        for (int r = 0; r < S; ++r) {
+          const uint2 other = maxima[r][lane];
+          m = make_uint2(join(m.x, other.x), join(m.y, other.y));
+        }
+        uint32_t most[W];
+        if constexpr (sizeof(T) == 2) {
+          most[0] = Mag<T>::lo(m.x);
+          most[1] = Mag<T>::hi(m.x);
+          most[2] = Mag<T>::lo(m.y);
+          most[3] = Mag<T>::hi(m.y);
+        } else {
+          most[0] = m.x;
+          most[1] = m.y;
+        }
+        TokenScale ts[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) ts[j].inverse = token_inverse(most[j]);
+        // this operand B's last product is done
+        const int q = groups > 1 ? group : turn & 1, use = groups > 1 ? turn : turn >> 1;
+        failed = use > 0 && !__all_sync(0xffffffffu, wait_or_abort(&sh.qempty[q], (uint32_t)((use - 1) & 1), abort));
+        if (failed) continue;
+        if (s == 0) {
+#pragma unroll
+          for (int j = 0; j < W; ++j) sh.scale[i % kI8MidScales][lane * W + j] = token_scale(most[j]).scale;
+        }
+        uint8_t* dst = qsm + q * q_bytes + (s >> 2) * (TOK * kI8BK) + lane * kI8BK;
+        constexpr int WH = W / 2;  // tokens of a word
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const TokenScale(&th)[WH] = *reinterpret_cast<const TokenScale(*)[WH]>(ts + half * WH);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t b[WH][4];
+            quantize16<T, WH>((half == 0 ? xa : xb) + h * 16, th, b);
+#pragma unroll
+            for (int j = 0; j < WH; ++j) {
+              const uint32_t keep = most[half * WH + j] >= 0x7f800000u ? 0u : 0xffffffffu;
+              *reinterpret_cast<uint4*>(dst + (half * WH + j) * (32 * kI8BK) + ((((s & 3) * 2 + h) ^ (lane & 7)) << 4)) =
+                  make_uint4(b[j][0] & keep, b[j][1] & keep, b[j][2] & keep, b[j][3] & keep);
+            }
+          }
+        }
+        fence_async_smem();
+        mbar_arrive(&sh.qfull[q]);
+        load(i + groups);
+      }
+    }
+  }
+  __syncthreads();
+  if (*abort && lane == 0) {
+    if (warp == 0) mbar_wait(&sh.weights, 0);
+    if (warp == 1) drain_mma(&sh.drain);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_cols);
+  }
+}
+
+// Groups of quantising warps (one warp per 32 channels): as many as there is room for.  False: not even one.
+bool mid_plan(int K, int N, int tok, int warps, int epi, int* groups, size_t* smem) {
+  const size_t kblocks = (K + kI8BK - 1) / kI8BK, mt = (N + kI8BM - 1) / kI8BM;
+  for (int g = std::min(kI8MidGroups, warps / ((K + 31) / 32)); g >= 1; --g) {
+    *groups = g;
+    *smem = kblocks * (mt * kI8BM + std::max(2, g) * tok) * kI8BK + (size_t)epi * kI8StageBytes + 1024;
+    if (*smem <= 227 * 1024 - sizeof(I8MidShared)) return true;
+  }
+  return false;
+}
+// Whether the medium form takes a product: whole 16-byte rows of y, room, and tiles enough for the SMs (108
+// tiles: 192 -> 64 7.9 us, two kernels 9.9, but 96 -> 32 9.0, 8.5).
+bool mid_takes(const void* x, const void* y, long long outer, int K, long long inner, int N, size_t esz) {
+  const int tok = 256 / (int)esz;
+  const long long tiles = outer * ((inner + tok - 1) / tok);
+  int groups;
+  size_t smem;
+  return K <= kI8MidK && N <= 4 * kI8BM && inner % (16 / (long long)esz) == 0 && reinterpret_cast<uintptr_t>(x) % 8 == 0 &&
+         reinterpret_cast<uintptr_t>(y) % 16 == 0 && mid_plan(K, N, tok, 8, 8, &groups, &smem) &&
+         tiles >= (K > 96 ? 64 : kI8Sms) && tiles < ((long long)1 << 30);
+}
+
+template <typename T>
+int launch_mid(const void* x, const int8_t* w, const float* ws, long long w_pitch, const float* bias, void* y,
+               long long outer, int K, long long inner, int N, cudaStream_t s) {
+  constexpr int tok = 256 / (int)sizeof(T);
+  I8GemmArgs p{};
+  p.a_scale = ws;
+  p.bias = bias;
+  p.y = y;
+  p.a_rows = N;
+  p.b_rows = (int)inner;
+  p.K = K;
+  p.N = N;
+  p.bn = tok;
+  p.a_tiles = (N + kI8BM - 1) / kI8BM;
+  p.b_tiles = (int)((inner + tok - 1) / tok);
+  p.samples = (int)outer;
+  p.accs = std::min(kI8MaxAcc, 512 / (p.a_tiles * tok));
+  p.copies = N <= 32 ? 4 : (N <= 64 ? 2 : 1);
+  CUtensorMap mW, mY;
+  if (!tma::encode_rows_8bit(&mW, w, K, N, 1, w_pitch, kI8BM / p.copies) ||
+      !tma::encode3<T>(&mY, y, inner, N, outer, tok / 2, 32, CU_TENSOR_MAP_SWIZZLE_128B)) {
+    note_cuda_error(cudaErrorInvalidValue);
+    return MEDNEXT_ERR_CUDA;
+  }
+  const auto run = [&](auto kern, int warps, int epi) {
+    size_t smem;
+    if (!mid_plan(K, N, tok, warps, epi, &p.groups, &smem)) return (int)MEDNEXT_ERR_BAD_SHAPE;
+    const int st = ensure_smem(kern, smem);
+    if (st != MEDNEXT_OK) return st;
+    const long long tiles = (long long)p.b_tiles * outer;
+    kern<<<(unsigned)std::min<long long>(tiles, num_sms()), 32 * (2 + epi + warps), smem, s>>>(static_cast<const T*>(x), mW, mY,
+                                                                                               p);
+    return record_launch();
+  };
+  // few outputs leave the work to the quantising warps (64^3, bf16: 192 -> 64 40 us, with 10 and 8 warps 52),
+  // many to the storing ones (128 -> 512 94 us, with 12 and 4 warps 117)
+  return N <= 64 ? run(i8_mid_kernel<T, 12, 4>, 12, 4) : run(i8_mid_kernel<T, 10, 8>, 10, 8);
+}
+
 // q: [outer * inner][q_pitch], w: [N][w_pitch]; y [outer, N, inner]
 template <typename T>
 int launch_gemm(const int8_t* q, const float* qs, long long q_pitch, const int8_t* w, const float* ws,
@@ -1780,6 +2126,8 @@ int launch_linear(const void* x, const int8_t* w, const float* ws, long long w_p
     c.inner = (int)inner; c.K = K; c.N = N;
     return launch_cluster<T>(c, w, w_pitch, outer, s);
   }
+  if (inner > 1 && mid_takes(x, y, outer, K, inner, N, sizeof(T)))
+    return launch_mid<T>(x, w, ws, w_pitch, bias, y, outer, K, inner, N, s);
   int st = launch_quantize<T>(x, q, qs, outer, K, inner, pitch16(K), s);
   if (st != MEDNEXT_OK) return st;
   return launch_gemm<T>(q, qs, pitch16(K), w, ws, w_pitch, bias, y, outer, inner, K, N, s);

@@ -344,3 +344,31 @@ def test_long_tokens_are_the_same_bits_in_any_company():
     stream.synchronize()
     assert all(torch.equal(a, y[:64]) for a in again)
     assert nat.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("outer,k,v,n", [
+    (1, 192, 12000, 64), (2, 100, 8192, 100), (1, 256, 9480, 256), (1, 128, 10000, 512), (3, 65, 3208, 129), (1, 40, 20000, 300),
+    (1, 250, 9608, 200), (40, 97, 264, 31), (1, 129, 30008, 384), (200, 70, 8, 16), (2, 160, 24 * 1000, 1),
+])
+def test_many_voxels_of_medium_width(outer, k, v, n, dtype):
+    w, s, b = weights(n, k, seed=v, pad=16)
+    check(activations((outer, k, v), dtype, seed=n), w, s, b, 1)
+    check(activations((outer, k, v), dtype, seed=n), w, s, None, 1)
+
+
+def test_voxels_of_medium_width_zero_or_not_finite_and_the_same_bits():
+    w, s, b = weights(96, 192, seed=9)
+    x = activations((1, 192, 20000), torch.float16, seed=10)
+    x[0, :, 5] = 0
+    x[0, 191, 77] = float("inf")
+    x[0, 0, 19999] = float("nan")
+    y = mx.int8_linear(x, w, s, b, dim=1)
+    bad = torch.tensor([77, 19999], device="cuda")
+    good = torch.ones(20000, dtype=torch.bool, device="cuda")
+    good[bad] = False
+    assert y[0][:, bad].isnan().all() and y[0][:, good].isfinite().all() and torch.equal(y[0, :, 5], b.half())
+    assert torch.equal(mx.int8_linear(x[0].t().contiguous(), w, s, b)[good], y[0].t()[good])  # the rows' form
+    for _ in range(20):
+        assert torch.equal(mx.int8_linear(x, w, s, b, dim=1)[0][:, good], y[0][:, good])
+    assert nat.device_error() == 0
