@@ -383,11 +383,55 @@ __device__ __forceinline__ void group_sum(float (&v)[N], int G, float* red, int&
 
 constexpr int kRowThreads = 256;
 
+// Rows of 16-bit data of odd width start at any element, and a warp's single elements are 64-byte
+// pieces off their sectors: 1.4 TB/s whatever the elements per thread (8, 16 or 32).  A CTA's rows are one
+// block of memory, though: with enough of them it goes through shared memory in 16-byte words, and
+// the threads take their elements from there.  An element lies as far from a 16-byte boundary in
+// shared memory as in global memory.
+template <typename T, int VEC, int R>
+constexpr bool kBlockRows = VEC == 1 && sizeof(T) == 2 && R > 1;
+template <typename T>
+__host__ __device__ __forceinline__ int block_bytes(int rows, int C) {
+  return (rows * C * (int)sizeof(T) + 31) / 16 * 16;
+}
+template <typename T>
+struct RowBlock {
+  static constexpr int E = 16 / (int)sizeof(T);
+  // the block's first element in shared memory
+  static __device__ __forceinline__ T* first(uint8_t* sm, const T* g) {
+    return reinterpret_cast<T*>(sm + (reinterpret_cast<uintptr_t>(g) & 15));
+  }
+  // f16(i): elements i .. i + E - 1, whole words of both sides; f1(i): single ones at the ends
+  template <typename F16, typename F1>
+  static __device__ __forceinline__ void each(const T* g, int n, F16 f16, F1 f1) {
+    const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(g) & 15)) & 15) / (int)sizeof(T));
+    const int words = (n - head) / E, tail = head + words * E;
+    for (int i = threadIdx.x; i < words; i += blockDim.x) f16(head + i * E);
+    if ((int)threadIdx.x < head) f1((int)threadIdx.x);
+    if ((int)threadIdx.x < n - tail) f1(tail + (int)threadIdx.x);
+  }
+  // asynchronously; arrived() waits for this thread's, a barrier follows
+  static __device__ __forceinline__ void fetch(uint8_t* sm, const T* g, int n) {
+    T* s = first(sm, g);
+    each(
+        g, n,
+        [=](int i) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(s + i)), "l"(g + i) : "memory"); },
+        [=](int i) { s[i] = g[i]; });
+  }
+  static __device__ __forceinline__ void arrived() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+  static __device__ __forceinline__ void put(T* g, uint8_t* sm, int n) {
+    const T* s = first(sm, g);
+    each(
+        g, n, [=](int i) { *reinterpret_cast<uint4*>(g + i) = *reinterpret_cast<const uint4*>(s + i); },
+        [=](int i) { g[i] = s[i]; });
+  }
+};
+
 // The next rows are on their way while a group works on its rows: a group is one or a few
 // warps, too few per SM to hide the loads' latency by their number.  Bound by HBM on long
 // rows (4096 x 4096 fp32: 25 us, 5.4 TB/s), by latency and start-up on few or short ones
 // (16384 x 1024 bf16: 17.8 us, 3.8 TB/s); single-element words by instruction issue
-// (30000 x 777 bf16: 61 us, 1.5 TB/s).
+// (30000 x 777 bf16: 50 us, 1.9 TB/s; without RowBlock 62).
 template <typename T, int VEC, int EPT, int R>
 __global__ void __launch_bounds__(kRowThreads, 2) ln_rows_fwd_kernel(LnArgs a, int G) {
   using Frag = RowFrag<T, VEC, EPT>;
@@ -399,7 +443,17 @@ __global__ void __launch_bounds__(kRowThreads, 2) ln_rows_fwd_kernel(LnArgs a, i
   const float rc = 1.f / (float)a.C;
   const long long stride = (long long)gridDim.x * groups * R;
   Frag next[R];
+  // (block rows: [2] blocks of x, a block of y)
+  constexpr bool kBlock = kBlockRows<T, VEC, R>;
+  uint8_t* block = reinterpret_cast<uint8_t*>(ln_sm);
+  const int bytes = block_bytes<T>(groups * R, a.C);
+  int buf = 0;
+  const auto of_block = [&](long long base) { return (int)min((long long)groups * R, a.tokens - base) * a.C; };
   const auto load = [&](long long base) {
+    if constexpr (kBlock) {
+      if (base < a.tokens) RowBlock<T>::fetch(block + buf * bytes, static_cast<const T*>(a.x) + base * a.C, of_block(base));
+      return;
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const long long t = base + r * groups + gi;
@@ -414,8 +468,18 @@ __global__ void __launch_bounds__(kRowThreads, 2) ln_rows_fwd_kernel(LnArgs a, i
   for (long long base = (long long)blockIdx.x * groups * R; base < a.tokens; base += stride) {
     Frag x[R];
     float s[R];
+    if constexpr (kBlock) {
+      RowBlock<T>::arrived();
+      __syncthreads();  // the block is there, the last block of y has been stored
+      const T* xs = RowBlock<T>::first(block + buf * bytes, static_cast<const T*>(a.x) + base * a.C);
 #pragma unroll
-    for (int r = 0; r < R; ++r) x[r] = next[r];
+      for (int r = 0; r < R; ++r)
+        x[r].load(xs + (r * groups + gi) * a.C, gl, G, a.C, base + r * groups + gi < a.tokens);
+      buf ^= 1;
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) x[r] = next[r];
+    }
     if (base + stride < a.tokens) load(base + stride);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -454,6 +518,8 @@ __global__ void __launch_bounds__(kRowThreads, 2) ln_rows_fwd_kernel(LnArgs a, i
       x[r].again();
       const float rstd = rsqrtf(s[r] * rc + a.eps);
       T* y = static_cast<T*>(a.y) + t * a.C;
+      if constexpr (kBlock)
+        y = RowBlock<T>::first(block + 2 * bytes, static_cast<T*>(a.y) + base * a.C) + (r * groups + gi) * a.C;
 #pragma unroll
       for (int j = 0; j < Frag::kChunks; ++j) {
         float2 f[Frag::kPairs], pw[Frag::kPairs], pb[Frag::kPairs];
@@ -465,6 +531,10 @@ __global__ void __launch_bounds__(kRowThreads, 2) ln_rows_fwd_kernel(LnArgs a, i
         Frag::store(y, j, gl, G, a.C, f);
       }
       if (a.stats != nullptr && gl == 0) a.stats[t] = make_float2(-nm[r].x, rstd);
+    }
+    if constexpr (kBlock) {
+      __syncthreads();
+      RowBlock<T>::put(static_cast<T*>(a.y) + base * a.C, block + 2 * bytes, of_block(base));
     }
   }
 }
@@ -487,11 +557,27 @@ __global__ void __launch_bounds__(kRowThreads, 2) ln_rows_bwd_kernel(LnArgs a, i
   const long long stride = (long long)gridDim.x * groups * R;
   Frag xn[R], dn[R];
   float2 stn[R];
+  // (block rows: [2] blocks of x, of dy, a block of dx)
+  constexpr bool kBlock = kBlockRows<T, VEC, R>;
+  uint8_t* block = reinterpret_cast<uint8_t*>(ln_sm);
+  const int bytes = block_bytes<T>(groups * R, a.C);
+  int buf = 0;
+  const auto of_block = [&](long long base) { return (int)min((long long)groups * R, a.tokens - base) * a.C; };
   const auto load = [&](long long base) {
+    if constexpr (kBlock) {
+      if (base < a.tokens) {
+        RowBlock<T>::fetch(block + buf * bytes, static_cast<const T*>(a.x) + base * a.C, of_block(base));
+        RowBlock<T>::fetch(block + (2 + buf) * bytes, static_cast<const T*>(a.dy) + base * a.C, of_block(base));
+      }
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const long long t = base + r * groups + gi;
       const bool in = t < a.tokens;
+      if constexpr (kBlock) {
+        stn[r] = in ? a.stats[t] : make_float2(0.f, 0.f);
+        continue;
+      }
       xn[r].load(static_cast<const T*>(a.x) + t * a.C, gl, G, a.C, in);
       dn[r].load(static_cast<const T*>(a.dy) + t * a.C, gl, G, a.C, in);
       stn[r] = in ? a.stats[t] : make_float2(0.f, 0.f);
@@ -509,11 +595,26 @@ __global__ void __launch_bounds__(kRowThreads, 2) ln_rows_bwd_kernel(LnArgs a, i
     float2 st[R];
     float s[2 * R];
     if (!kAhead) load(base);
+    if constexpr (kBlock) {
+      RowBlock<T>::arrived();
+      __syncthreads();  // the blocks are there, the last block of dx has been stored
+      const T* xs = RowBlock<T>::first(block + buf * bytes, static_cast<const T*>(a.x) + base * a.C);
+      const T* ds = RowBlock<T>::first(block + (2 + buf) * bytes, static_cast<const T*>(a.dy) + base * a.C);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      x[r] = xn[r];
-      d[r] = dn[r];
-      st[r] = stn[r];
+      for (int r = 0; r < R; ++r) {
+        const bool in = base + r * groups + gi < a.tokens;
+        x[r].load(xs + (r * groups + gi) * a.C, gl, G, a.C, in);
+        d[r].load(ds + (r * groups + gi) * a.C, gl, G, a.C, in);
+        st[r] = stn[r];
+      }
+      buf ^= 1;
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        x[r] = xn[r];
+        d[r] = dn[r];
+        st[r] = stn[r];
+      }
     }
     if (kAhead && base + stride < a.tokens) load(base + stride);
 #pragma unroll
@@ -546,6 +647,8 @@ __global__ void __launch_bounds__(kRowThreads, 2) ln_rows_bwd_kernel(LnArgs a, i
       d[r].again();
       const float2 m1 = f2(-s[2 * r] * rc), m2 = f2(-s[2 * r + 1] * rc);
       T* dx = static_cast<T*>(a.y) + t * a.C;
+      if constexpr (kBlock)
+        dx = RowBlock<T>::first(block + 4 * bytes, static_cast<T*>(a.y) + base * a.C) + (r * groups + gi) * a.C;
 #pragma unroll
       for (int j = 0; j < Frag::kChunks; ++j) {
         float2 f[Frag::kPairs], pw[Frag::kPairs];
@@ -560,6 +663,10 @@ __global__ void __launch_bounds__(kRowThreads, 2) ln_rows_bwd_kernel(LnArgs a, i
         Frag::store(dx, j, gl, G, a.C, f);
       }
     }
+    if constexpr (kBlock) {
+      __syncthreads();
+      RowBlock<T>::put(static_cast<T*>(a.y) + base * a.C, block + 4 * bytes, of_block(base));
+    }
   }
   if (a.part == nullptr) return;
   // lanes of one warp that hold the same columns, then the CTA's slots, in order
@@ -571,7 +678,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) ln_rows_bwd_kernel(LnArgs a, i
       db[i].x += __shfl_xor_sync(0xffffffffu, db[i].x, o);
       db[i].y += __shfl_xor_sync(0xffffffffu, db[i].y, o);
     }
-  __syncthreads();  // the parameters in shared memory give way
+  __syncthreads();  // the parameters or blocks in shared memory give way
   const int slot = G < 32 ? threadIdx.x >> 5 : gi, slots = G < 32 ? blockDim.x >> 5 : groups;
   if (G >= 32 || (threadIdx.x & 31) < G) {
 #pragma unroll
@@ -1123,15 +1230,17 @@ int launch_rows(const LnArgs& a, const LnPlan& p, bool bwd, int parts, cudaStrea
   const size_t param = RowParam<T, VEC, EPT>::smem_bytes(p.G);
   if (!bwd) {
     auto kern = ln_rows_fwd_kernel<T, VEC, EPT, R>;
-    const int st = ensure_smem(kern, 2 * param);
+    const size_t smem = kBlockRows<T, VEC, R> ? 3 * (size_t)block_bytes<T>(p.threads / p.G * R, a.C) : 2 * param;
+    const int st = ensure_smem(kern, smem);
     if (st != MEDNEXT_OK) return st;
     const long long cap = kSms * 2LL;  // resident by the launch bounds
-    kern<<<(unsigned)std::min((p.units + R - 1) / R, cap), p.threads, 2 * param, s>>>(a, p.G);
+    kern<<<(unsigned)std::min((p.units + R - 1) / R, cap), p.threads, smem, s>>>(a, p.G);
   } else {
     constexpr int RB = R > 2 ? 2 : 1;
     auto kern = ln_rows_bwd_kernel<T, VEC, EPT, RB>;
     const int slots = p.G < 32 ? p.threads / 32 : p.threads / p.G;
-    const size_t smem = std::max(param, a.part != nullptr ? (size_t)slots * 2 * a.C * sizeof(float) : 0);
+    const size_t held = kBlockRows<T, VEC, RB> ? 5 * (size_t)block_bytes<T>(p.threads / p.G * RB, a.C) : param;
+    const size_t smem = std::max(held, a.part != nullptr ? (size_t)slots * 2 * a.C * sizeof(float) : 0);
     const int st = ensure_smem(kern, smem);
     if (st != MEDNEXT_OK) return st;
     kern<<<parts, p.threads, smem, s>>>(a, p.G);

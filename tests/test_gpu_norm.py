@@ -334,3 +334,45 @@ def test_channels_first_wide(shape, dtype):
         check(x.transpose(1, 2).contiguous().transpose(1, 2), w, b, dy, 1)
         y = x.permute(1, 2, 0).contiguous().permute(2, 0, 1)
         check(y, w, b, dy, 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,c", [(9001, 1), (20011, 3), (30001, 31), (12007, 97), (7777, 333), (5003, 777), (4001, 2047)])
+def test_many_odd_rows_at_any_element(rows, c, dtype):
+    """Blocks of rows that start and end off every boundary, each tensor at its own element: the bits of aligned copies,
+    and within bounds of the 64-bit result."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    x = (torch.randn((rows, c), generator=gen, device="cuda") * 2 + 0.5).to(dtype)
+    dy = torch.randn((rows, c), generator=gen, device="cuda").to(dtype)
+    w = torch.randn(c, generator=gen, device="cuda")
+    b = torch.randn(c, generator=gen, device="cuda")
+
+    def at(t, off):
+        held = torch.full((t.numel() + 16,), 7.0, dtype=t.dtype, device="cuda")
+        view = held[off:off + t.numel()].view(t.shape)
+        view.copy_(t)
+        return view
+
+    results = []
+    for ox, od in ((0, 0), (1, 6), (5, 3)):
+        xs = at(x, ox).requires_grad_()
+        ws, bs = w.clone().requires_grad_(), b.clone().requires_grad_()
+        y = mx.layer_norm(xs, ws, bs)
+        results.append((y, *torch.autograd.grad(y, (xs, ws, bs), at(dy, od))))
+    for other in results[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(results[0], other))
+    x64 = x.double()
+    mean = x64.mean(1, keepdim=True)
+    rstd = (x64.var(1, unbiased=False, keepdim=True) + 1e-6).rsqrt()
+    xh = (x64 - mean) * rstd
+    want = xh * w.double() + b.double()
+    u = 2.0**-8 if dtype == torch.bfloat16 else 2.0**-11
+    size = want.abs() + xh.abs() * w.double().abs() + b.double().abs() + 1e-3
+    assert ((results[0][0].double() - want).abs() <= u * want.abs() + 2.0**-16 * size).all()
+    g = dy.double() * w.double()
+    dx = rstd * (g - g.mean(1, keepdim=True) - xh * (g * xh).mean(1, keepdim=True))
+    size = rstd * (g.abs() + g.abs().mean(1, keepdim=True) + xh.abs() * (g * xh).abs().mean(1, keepdim=True))
+    assert ((results[0][1].double() - dx).abs() <= u * dx.abs() + 2.0**-16 * size + 1e-7).all()
+    for got, terms in ((results[0][2], dy.double() * xh), (results[0][3], dy.double())):
+        assert ((got.double() - terms.sum(0)).abs() <= 2.0**-16 * terms.abs().sum(0) + 1e-6).all()
+    assert nat.device_error() == 0
