@@ -399,6 +399,45 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool ab_bf16
 __device__ __forceinline__ void grid_dependents_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// A block of rows that starts and ends at any element, through shared memory in 16-byte words: an
+// element lies as far from a 16-byte boundary there as in global memory.
+template <typename T>
+__host__ __device__ __forceinline__ int block_bytes(int rows, int C) {
+  return (rows * C * (int)sizeof(T) + 31) / 16 * 16;
+}
+template <typename T>
+struct RowBlock {
+  static constexpr int E = 16 / (int)sizeof(T);
+  // the block's first element in shared memory
+  static __device__ __forceinline__ T* first(uint8_t* sm, const T* g) {
+    return reinterpret_cast<T*>(sm + (reinterpret_cast<uintptr_t>(g) & 15));
+  }
+  // f16(i): elements i .. i + E - 1, whole words of both sides; f1(i): single ones at the ends
+  template <typename F16, typename F1>
+  static __device__ __forceinline__ void each(const T* g, int n, F16 f16, F1 f1) {
+    const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(g) & 15)) & 15) / (int)sizeof(T));
+    const int words = (n - head) / E, tail = head + words * E;
+    for (int i = threadIdx.x; i < words; i += blockDim.x) f16(head + i * E);
+    if ((int)threadIdx.x < head) f1((int)threadIdx.x);
+    if ((int)threadIdx.x < n - tail) f1(tail + (int)threadIdx.x);
+  }
+  // asynchronously; arrived() waits for this thread's, a barrier follows
+  static __device__ __forceinline__ void fetch(uint8_t* sm, const T* g, int n) {
+    T* s = first(sm, g);
+    each(
+        g, n,
+        [=](int i) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(s + i)), "l"(g + i) : "memory"); },
+        [=](int i) { s[i] = g[i]; });
+  }
+  static __device__ __forceinline__ void arrived() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+  static __device__ __forceinline__ void put(T* g, uint8_t* sm, int n) {
+    const T* s = first(sm, g);
+    each(
+        g, n, [=](int i) { *reinterpret_cast<uint4*>(g + i) = *reinterpret_cast<const uint4*>(s + i); },
+        [=](int i) { g[i] = s[i]; });
+  }
+};
+
 // 2^x and 1/x by the PTX approximate instructions (relative error about 2^-22;
 // denormal results flush to zero).
 __device__ __forceinline__ float ex2_approx(float x) {

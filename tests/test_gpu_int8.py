@@ -372,3 +372,20 @@ def test_voxels_of_medium_width_zero_or_not_finite_and_the_same_bits():
     for _ in range(20):
         assert torch.equal(mx.int8_linear(x, w, s, b, dim=1)[0][:, good], y[0][:, good])
     assert nat.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,k,off", [(9473, 777, 0), (12001, 33, 1), (20000, 1023, 3), (9472, 5, 7), (10007, 96, 5), (30000, 1, 0)])
+def test_many_odd_rows_are_quantised_alike(t, k, off, dtype):
+    """Rows off every boundary, in blocks: the formula's bytes."""
+    x = activations((t, k), dtype, seed=k)
+    held = torch.empty(x.numel() + 8, dtype=dtype, device="cuda")
+    view = held[off:off + x.numel()].view(t, k)
+    view.copy_(x)
+    view[17] = 0
+    view[t - 1, k - 1] = float("inf")
+    q, s = mx.quantize_int8(view)
+    wq, ws = quantized(view, 1)
+    assert torch.equal(q[:-1].float(), wq[:-1]) and torch.equal(s[:-1], ws[:-1])
+    assert not q[-1].any() and s[-1].isinf()
+    assert nat.device_error() == 0
