@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(1024) i8_quantize_chan_kernel(const T* __restr
 // lane and step, so that their bytes are one store.  128 kSteps values stay in registers;
 // longer rows are read again (from L1 / L2) to be scaled.
 // BLOCK: eight rows of 16-bit data at a time through shared memory, the next eight under way
-// (100000 x 777 fp16: 65 us, from global memory 76 to 98; 10000 x 97 4.3, 3.6).
+// (100000 x 777 fp16: 66 us, from global memory 77; 30000 x 2001 bf16 53, 75; 10000 x 97 4.3, 3.6).
 template <typename T, bool BLOCK, int kSteps>
 __global__ void __launch_bounds__(256) i8_quantize_any_kernel(const T* __restrict__ x, int8_t* __restrict__ q,
                                                               float* __restrict__ scale, long long tokens, int K,
@@ -270,14 +270,14 @@ __global__ void __launch_bounds__(256) i8_quantize_any_kernel(const T* __restric
   };
   if (BLOCK) fetch((long long)blockIdx.x * 8);
   // the CTA's warps go their own ways, or together from block to block
-  const int first = BLOCK ? 0 : threadIdx.x >> 5;
-  for (long long t0 = (long long)blockIdx.x * 8; t0 + first < tokens; t0 += (long long)gridDim.x * 8) {
-    const long long t = t0 + (threadIdx.x >> 5);
+  const int warp = threadIdx.x >> 5;
+  for (long long t = (long long)blockIdx.x * 8 + warp; (BLOCK ? t - warp : t) < tokens; t += (long long)gridDim.x * 8) {
     const T* p = x + t * K;
     if constexpr (BLOCK) {
+      const long long t0 = t - warp;
       RowBlock<T>::arrived();
       __syncthreads();  // this block is there, the last one has been read
-      p = RowBlock<T>::first(i8_rows + buf * bytes, x + t0 * K) + (threadIdx.x >> 5) * K;
+      p = RowBlock<T>::first(i8_rows + buf * bytes, x + t0 * K) + warp * K;
       buf ^= 1;
       fetch(t0 + (long long)gridDim.x * 8);
       if (t >= tokens) continue;
@@ -2096,9 +2096,12 @@ int launch_quantize(const void* xv, int8_t* q, float* scale, long long outer, in
   const auto any = [&](auto steps) {
     constexpr int kSteps = decltype(steps)::value;
     if constexpr (sizeof(T) == 2 && kSteps >= 4)
-      if (K <= 1024 && tokens >= kI8Sms * 64LL) {  // several blocks for each resident CTA
-        i8_quantize_any_kernel<T, true, kSteps><<<kI8Sms * (kSteps < 8 ? 4 : 2), 256, 2 * (size_t)block_bytes<T>(8, K), s>>>(
-            x, q, scale, tokens, K, (int)pitch);
+      if (K <= 2048 && tokens >= kI8Sms * 64LL) {  // several blocks for each resident CTA
+        const size_t smem = 2 * (size_t)block_bytes<T>(8, K);
+        const int st = ensure_smem(i8_quantize_any_kernel<T, true, kSteps>, smem);
+        if (st != MEDNEXT_OK) return st;
+        i8_quantize_any_kernel<T, true, kSteps><<<kI8Sms * (kSteps < 8 ? 4 : 2), 256, smem, s>>>(x, q, scale, tokens, K,
+                                                                                                 (int)pitch);
         return record_launch();
       }
     i8_quantize_any_kernel<T, false, kSteps><<<(unsigned)std::min<long long>((tokens + 7) / 8, kI8Sms * 16), 256, 0, s>>>(

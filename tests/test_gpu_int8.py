@@ -375,7 +375,7 @@ def test_voxels_of_medium_width_zero_or_not_finite_and_the_same_bits():
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("t,k,off", [(9473, 777, 0), (12001, 33, 1), (20000, 1023, 3), (9472, 5, 7), (10007, 96, 5), (30000, 1, 0)])
+@pytest.mark.parametrize("t,k,off", [(9473, 777, 0), (12001, 33, 1), (20000, 1023, 3), (9999, 1301, 5), (9500, 2047, 1), (9480, 2049, 0), (9472, 5, 7), (10007, 96, 5), (30000, 1, 0)])
 def test_many_odd_rows_are_quantised_alike(t, k, off, dtype):
     """Rows off every boundary, in blocks: the formula's bytes."""
     x = activations((t, k), dtype, seed=k)
