@@ -326,8 +326,8 @@ __global__ void __launch_bounds__(256) i8_quantize_any_kernel(const T* __restric
 // Persistent, warp-specialised: warp 0 issues the TMA loads (a ring of 128-byte K
 // blocks), warp 1 owns TMEM and issues the MMAs into two to four accumulators in turn, two
 // groups of four warps scale and store: a tile each in turn where TMEM holds four, so that one
-// tile's latencies pass under the other's, else half of every tile each.  The waits and the exit follow the pointwise kernels' discipline: every wait
-// is bounded, and what is in flight is waited for before TMEM is freed.
+// tile's latencies pass under the other's, else half of every tile each.  The waits and the exit follow
+// the pointwise kernels' discipline: every wait is bounded, and what is in flight is waited for before TMEM is freed.
 constexpr int kI8BM = 128, kI8BK = 128;
 constexpr int kI8Threads = 320, kI8EpiWarps = 8;
 constexpr int kI8MaxStages = 8, kI8MaxAcc = 4;
@@ -1055,7 +1055,8 @@ size_t narrow_smem(int K, int N, int W, int P) {
   return (size_t)narrow_weight_bytes(K, N) + (size_t)P * (narrow_tile_bytes(K, W) + S * mt_store * kNarrowStage) + 1024;
 }
 // Whether the one-kernel form takes a product: K and N small enough that bytes are its bound
-// (bf16, 64^3 voxels: 64 -> 192 channels 42 us against 51 us in two kernels; wider ones go to the medium form), whole 16-byte rows, and enough tiles.
+// (bf16, 64^3 voxels: 64 -> 192 channels 42 us against 51 us in two kernels; wider ones go to the
+// medium form), whole 16-byte rows, and enough tiles.
 bool narrow_takes(const void* x, const void* y, long long outer, int K, long long inner, int N, size_t esz) {
   return K <= 64 && N <= 256 && inner % (16 / (long long)esz) == 0 && reinterpret_cast<uintptr_t>(x) % 4 == 0 &&
          reinterpret_cast<uintptr_t>(y) % 16 == 0 && outer * ((inner + 63) / 64) >= 2 * kI8Sms;
