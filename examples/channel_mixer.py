@@ -12,6 +12,7 @@ their predictions compared with the 16-bit ones.
 from __future__ import annotations
 
 import argparse
+import copy
 import sys
 from pathlib import Path
 
@@ -36,7 +37,7 @@ class MixerNet(nn.Module):
 
     def int8(self) -> MixerNet:
         served = MixerNet(depth=0)
-        served.head = self.head
+        served.head = copy.deepcopy(self.head).requires_grad_(False)
         served.mixers = nn.ModuleList(mixer.int8() for mixer in self.mixers)
         return served.eval()
 

@@ -12,6 +12,8 @@ dropout.
 
 from __future__ import annotations
 
+import copy
+
 import torch
 from torch import Tensor, nn
 from torch.nn import functional as F
@@ -55,7 +57,8 @@ class ChannelMixer3d(nn.Module):
         return dropout(y, self.p, rng, residual=x, layer=self.layer)
 
     def int8(self) -> Int8ChannelMixer3d:
-        """The serving form of the mixer as it is now (its weights are quantised)."""
+        """The serving form of the mixer as it is now: its weights are quantised, its norm is
+        copied, and neither form follows what becomes of the other."""
         return Int8ChannelMixer3d(self)
 
 
@@ -64,7 +67,7 @@ class Int8ChannelMixer3d(nn.Module):
 
     def __init__(self, mixer: ChannelMixer3d) -> None:
         super().__init__()
-        self.norm = mixer.norm
+        self.norm = copy.deepcopy(mixer.norm).requires_grad_(False)
         self.expand = Int8Pointwise3d(mixer.expand)
         self.project = Int8Pointwise3d(mixer.project)
 

@@ -99,3 +99,51 @@ def test_example_trains_and_serves():
     assert losses[-1] < 0.8 * losses[0]
     full, low, same = example.compare(net, x, target)
     assert full > 0.5 and same > 0.95 and abs(full - low) < 0.03
+
+
+def step(module, x, lr=0.1):
+    """One optimiser step that moves every parameter."""
+    opt = torch.optim.SGD(module.parameters(), lr=lr)
+    y = module(x)
+    (y.float() * torch.linspace(-1, 1, y.numel(), device=y.device).view_as(y)).sum().backward()
+    before = [p.detach().clone() for p in module.parameters()]
+    opt.step()
+    assert all(not torch.equal(p, q) for p, q in zip(before, module.parameters(), strict=True))
+
+
+def test_served_mixer_does_not_follow_the_trained_one():
+    torch.manual_seed(2)
+    mixer = mx.ChannelMixer3d(16, 2).cuda()
+    x = torch.randn((1, 16, 4, 6, 8), device="cuda").to(torch.bfloat16)
+    served = mixer.int8()
+    want = served(x)
+    step(mixer, x)
+    assert torch.equal(served(x), want)
+    assert not torch.equal(mixer.int8()(x), want)
+
+
+def test_trained_mixer_does_not_follow_the_served_one():
+    mixer = mx.ChannelMixer3d(16, 2).cuda()
+    x = torch.randn((1, 16, 4, 6, 8), device="cuda")
+    step(mixer, x)  # parameters with gradients
+    grads = [p.grad for p in mixer.parameters()]
+    served = mixer.int8()
+    assert not any(p.requires_grad or p.grad is not None for p in served.parameters())
+    served.bfloat16()
+    assert all(p.requires_grad and p.dtype == torch.float32 for p in mixer.parameters())
+    assert all(p.grad is g for p, g in zip(mixer.parameters(), grads, strict=True))
+
+
+def test_served_example_does_not_follow_the_trained_one():
+    path = Path(__file__).resolve().parents[1] / "examples" / "channel_mixer.py"
+    spec = importlib.util.spec_from_file_location("channel_mixer_example", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    net = example.MixerNet(p=0.0).cuda()
+    x, _ = example.synthetic(8)
+    served = net.int8()
+    with torch.no_grad():
+        want = served(x)
+    step(net, x)
+    with torch.no_grad():
+        assert torch.equal(served(x), want)
