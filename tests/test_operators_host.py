@@ -118,3 +118,16 @@ def test_tensors_on_the_cpu_are_refused():
         mx.quantize_int8(x)
     with pytest.raises(ValueError, match="positive"):
         mx.LayerNorm3d(0)
+
+
+def test_8_bit_convolutions_refuse_transposed_weights():
+    """A transposed convolution's weight is [in, out]: its rows are not the output channels."""
+    for cin, cout in ((8, 8), (4, 12)):
+        with pytest.raises(ValueError, match="1x1x1"):
+            mx.Int8Pointwise3d(torch.nn.ConvTranspose3d(cin, cout, 1))
+    head = mx.mednext_small(in_channels=1, out_channels=3, kernel_size=3)
+    heads = [m for m in head.modules() if getattr(m, "transposed", False) and set(m.kernel_size) == {1}]
+    assert heads
+    for m in heads:
+        with pytest.raises(ValueError, match="1x1x1"):
+            mx.Int8Pointwise3d(m)
