@@ -127,7 +127,11 @@ def int8_linear(x: Tensor, weight: Tensor, scale: Tensor, bias: Tensor | None = 
 
 
 class Int8Pointwise3d(nn.Module):
-    """An ``nn.Conv3d`` with a 1x1x1 kernel, served in 8-bit integers."""
+    """An ``nn.Conv3d`` with a 1x1x1 kernel, served in 8-bit integers.
+
+    Its 8-bit rows, float32 scales and float32 bias keep their types and values when the
+    module, or a model that holds it, is cast (``.half()``, ``.to(dtype)``): the products
+    take x in any of its types and these as they are."""
 
     def __init__(self, conv: nn.Conv3d) -> None:
         super().__init__()
@@ -142,6 +146,15 @@ class Int8Pointwise3d(nn.Module):
         self.register_buffer("weight", q.as_strided((conv.out_channels, pitch), (pitch, 1)))
         self.register_buffer("scale", scale)
         self.register_buffer("bias", None if conv.bias is None else conv.bias.detach().float().clone())
+
+    def _apply(self, fn, recurse=True):
+        held = dict(self._buffers)
+        super()._apply(fn, recurse)
+        for name, t in held.items():
+            now = self._buffers[name]
+            if t is not None and now.dtype != t.dtype:
+                self._buffers[name] = t.to(now.device)
+        return self
 
     def forward(self, x: Tensor) -> Tensor:
         return int8_linear(x, self.weight[:, : self.in_channels], self.scale, self.bias, dim=1)

@@ -389,3 +389,22 @@ def test_many_odd_rows_are_quantised_alike(t, k, off, dtype):
     assert torch.equal(q[:-1].float(), wq[:-1]) and torch.equal(s[:-1], ws[:-1])
     assert not q[-1].any() and s[-1].isinf()
     assert nat.device_error() == 0
+
+
+@pytest.mark.parametrize("cast", [
+    lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.double(), lambda m: m.to(torch.float16), lambda m: m.type(torch.half),
+    lambda m: m.to("cpu", torch.bfloat16).cuda(),
+])
+def test_a_cast_module_keeps_its_numbers(cast):
+    """The 8-bit rows, their fp32 scales and the fp32 bias are what the products take, whatever the model is cast to."""
+    torch.manual_seed(0)
+    model = torch.nn.Sequential(mx.Int8Pointwise3d(torch.nn.Conv3d(24, 40, 1).cuda()))
+    x = activations((1, 24, 4, 5, 6), torch.float16)
+    want = model(x)
+    held = {name: t.clone() for name, t in model.state_dict().items()}
+    model = cast(model)
+    for name, t in model.state_dict().items():
+        assert t.is_cuda and t.dtype == held[name].dtype and torch.equal(t, held[name]), name
+    assert torch.equal(model(x), want)
+    without = cast(mx.Int8Pointwise3d(torch.nn.Conv3d(24, 40, 1, bias=False).cuda()))
+    assert without.bias is None and without(x).shape == want.shape

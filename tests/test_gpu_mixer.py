@@ -147,3 +147,17 @@ def test_served_example_does_not_follow_the_trained_one():
     step(net, x)
     with torch.no_grad():
         assert torch.equal(served(x), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_served_mixer_can_be_cast(dtype):
+    """The norm's parameters are rounded to the new type, up to 2^-8 each: rows within 2e-2 as above."""
+    mixer = mx.ChannelMixer3d(32, 2).cuda()
+    with torch.no_grad():
+        mixer.norm.weight.uniform_(0.5, 1.5)
+    x = torch.randn((1, 32, 4, 6, 8), device="cuda").to(dtype)
+    served = mixer.int8()
+    want = served(x).float() - x.float()
+    served.to(dtype)
+    assert served.norm.weight.dtype == dtype
+    assert rel(served(x).float() - x.float(), want) <= 2e-2
