@@ -32,9 +32,12 @@ def _pointwise(x: Tensor, conv: nn.Conv3d) -> Tensor:
 
 
 class ChannelMixer3d(nn.Module):
-    """``forward(x, rng)``: x [N, C, D, H, W] in float32, bfloat16 or float16 (the branch runs
-    in x's type), ``rng`` the [seed, offset] tensor of :func:`dropout`, needed while training
-    with ``p > 0``.  ``layer`` tells the mixers of one model apart in their masks."""
+    """``forward(x, rng)``: x [N, C, D, H, W] in float32, bfloat16 or float16, ``rng`` the
+    [seed, offset] tensor of :func:`dropout`, needed while training with ``p > 0``.  ``layer``
+    tells the mixers of one model apart in their masks.
+
+    The branch runs in x's type and the result has it.  Under autocast the convolutions of
+    float32 or non-contiguous features, which are torch's, run in autocast's type."""
 
     def __init__(self, channels: int, expansion_ratio: int, p: float = 0.0, layer: int = 0) -> None:
         super().__init__()
@@ -49,7 +52,7 @@ class ChannelMixer3d(nn.Module):
         self.project = nn.Conv3d(channels * expansion_ratio, channels, kernel_size=1)
 
     def forward(self, x: Tensor, rng: Tensor | tuple[int, int] | None = None) -> Tensor:
-        y = _pointwise(F.gelu(_pointwise(self.norm(x), self.expand)), self.project)
+        y = _pointwise(F.gelu(_pointwise(self.norm(x), self.expand)), self.project).to(x.dtype)
         if not self.training or self.p == 0.0:
             return x + y
         if rng is None:

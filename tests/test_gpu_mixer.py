@@ -161,3 +161,45 @@ def test_served_mixer_can_be_cast(dtype):
     served.to(dtype)
     assert served.norm.weight.dtype == dtype
     assert rel(served(x).float() - x.float(), want) <= 2e-2
+
+
+def test_training_under_autocast_matches_64_bits():
+    """float32 features under bfloat16 autocast: the products in bfloat16, tolerances as for it above; what
+    dropout leaves out is exact."""
+    torch.manual_seed(0)
+    shape = (2, 24, 5, 6, 8)
+    mixer = mx.ChannelMixer3d(shape[1], 2, p=0.25, layer=3).cuda().train()
+    x, dy = (torch.randn(shape, device="cuda") for _ in range(2))
+    xg = x.clone().requires_grad_()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = mixer(xg, torch.tensor([40, 2], device="cuda"))
+    assert y.dtype == torch.float32
+    grads = torch.autograd.grad(y, [xg, *mixer.parameters()], dy)
+    keep = torch.from_numpy(dropout_words(43, 2, 0, x.numel()) >= round(0.25 * 65536)).cuda().view(shape)
+    assert torch.equal(y[~keep], x[~keep])
+    want, xd, w = reference(mixer, x, keep, 0.25)
+    want_grads = torch.autograd.grad(want, [xd, *w.values()], dy.double())
+    assert rel(y, want) <= 2e-2
+    for (name, _), got, ref in zip([("x", None), *mixer.named_parameters()], grads, want_grads, strict=True):
+        assert got.dtype == torch.float32 and rel(got, ref) <= 2e-2, name
+    assert nat.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cast", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("memory_format", [torch.contiguous_format, torch.channels_last_3d])
+def test_features_keep_their_type_under_autocast(dtype, cast, memory_format):
+    torch.manual_seed(0)
+    mixer = mx.ChannelMixer3d(16, 2, p=0.5).cuda()
+    served = mixer.int8()
+    x = torch.randn((2, 16, 4, 6, 8), device="cuda").to(dtype).contiguous(memory_format=memory_format)
+    want, _, _ = reference(mixer, x, None, 0.5)
+    with torch.autocast("cuda", dtype=cast):
+        mixer.train()
+        y = mixer(x, (1, 2))
+        mixer.eval()
+        z, low = mixer(x), served(x)
+    assert y.dtype == z.dtype == low.dtype == dtype
+    assert rel(z, want) <= 2e-2 and rel(low, want) <= 3e-2
+    y.float().sum().backward()
+    assert all(p.grad is not None and p.grad.isfinite().all() for p in mixer.parameters())
