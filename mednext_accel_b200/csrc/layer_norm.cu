@@ -141,9 +141,9 @@ __device__ __forceinline__ void store_param(void* p, int dtype, int i, double v)
 }
 
 // dw, db = the partials' sums in a fixed order: 32 warps take every 32nd part of 32
-// columns, then one adds the 32 sums.  parts = 0 writes zeros (no tokens).
-__global__ void __launch_bounds__(1024) ln_fold_kernel(const float* __restrict__ part, int parts, int C, void* dw,
-                                                      void* db, int pdt) {
+// columns, then one adds the 32 sums.  parts = 0 writes zeros (no tokens).  part is plain memory
+// (not __restrict__, which would allow read-only loads): it is launched while part is written.
+__global__ void __launch_bounds__(1024) ln_fold_kernel(const float* part, int parts, int C, void* dw, void* db, int pdt) {
   __shared__ double red[2][32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;

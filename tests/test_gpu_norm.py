@@ -376,3 +376,18 @@ def test_many_odd_rows_at_any_element(rows, c, dtype):
     for got, terms in ((results[0][2], dy.double() * xh), (results[0][3], dy.double())):
         assert ((got.double() - terms.sum(0)).abs() <= 2.0**-16 * terms.abs().sum(0) + 1e-6).all()
     assert nat.device_error() == 0
+
+
+@pytest.mark.parametrize("shape,dim", [((3000, 256), 1), ((1, 32, 20000), 1), ((40, 9000), 1)])
+def test_the_fold_reads_the_partials_of_its_own_call(shape, dim):
+    """Calls in a row take the same workspace, and each fold starts while its partials are written: every call gives
+    the bits of a call on its own."""
+    x, w, b, dy = inputs(shape, dim, torch.bfloat16)
+    gradients = [dy, dy.neg(), dy * 3, dy.flip(0).contiguous()]
+    want = []
+    for g in gradients:
+        want.append(check_free(x, w, b, g, dim)[2:])
+        torch.cuda.synchronize()
+    results = [check_free(x, w, b, gradients[i % 4], dim)[2:] for i in range(60)]  # queued, not waited for
+    for i, got in enumerate(results):
+        assert all(torch.equal(p, q) for p, q in zip(got, want[i % 4], strict=True)), i
