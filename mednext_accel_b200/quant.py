@@ -137,7 +137,7 @@ class Int8Pointwise3d(nn.Module):
         super().__init__()
         transposed = getattr(conv, "transposed", False)  # its weight would be [in, out]
         if (transposed or conv.groups != 1 or set(conv.kernel_size) != {1} or set(conv.stride) != {1}
-                or set(conv.padding) != {0}):
+                or (conv.padding not in ("same", "valid") and set(conv.padding) != {0})):
             raise ValueError("Int8Pointwise3d requires a dense 1x1x1 convolution of stride 1 without padding, not transposed")
         q, scale = quantize_int8(conv.weight.reshape(conv.out_channels, conv.in_channels))
         # the padded rows are the buffer: a slice's row pitch would not survive a state dict

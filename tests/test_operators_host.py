@@ -131,3 +131,11 @@ def test_8_bit_convolutions_refuse_transposed_weights():
     for m in heads:
         with pytest.raises(ValueError, match="1x1x1"):
             mx.Int8Pointwise3d(m)
+
+
+@pytest.mark.parametrize("padding", ["same", "valid", 0, (0, 0, 0)])
+def test_8_bit_convolutions_take_every_way_to_say_no_padding(padding):
+    with pytest.raises(ValueError, match="CUDA"):  # nothing but the device is refused
+        mx.Int8Pointwise3d(torch.nn.Conv3d(4, 8, 1, padding=padding))
+    with pytest.raises(ValueError, match="1x1x1"):
+        mx.Int8Pointwise3d(torch.nn.Conv3d(4, 8, 1, padding=1))
