@@ -25,6 +25,8 @@ int record_launch() {
 int last_cuda_error() { return t_last_cuda_error; }
 void note_cuda_error(cudaError_t e) { t_last_cuda_error = (int)e; }
 
+constexpr size_t kDefaultSmem = 48 * 1024;  // a block's without an opt-in
+
 int ensure_smem_fn(const void* fn, size_t smem) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -33,9 +35,21 @@ int ensure_smem_fn(const void* fn, size_t smem) {
     return MEDNEXT_ERR_CUDA;
   }
   static std::mutex mu;
-  static std::map<std::pair<const void*, int>, size_t> granted;  // largest size granted per (kernel, device)
+  // per (kernel, device): the dynamic shared memory that a launch may ask for
+  static std::map<std::pair<const void*, int>, size_t> granted;
   std::lock_guard<std::mutex> lock(mu);
-  size_t& have = granted[{fn, dev}];
+  const auto [at, first] = granted.try_emplace({fn, dev}, 0);
+  size_t& have = at->second;
+  if (first) {
+    cudaFuncAttributes attr;
+    e = cudaFuncGetAttributes(&attr, fn);
+    if (e != cudaSuccess) {
+      granted.erase(at);
+      note_cuda_error(e);
+      return MEDNEXT_ERR_CUDA;
+    }
+    have = kDefaultSmem - std::min(kDefaultSmem, attr.sharedSizeBytes);
+  }
   if (smem <= have) return MEDNEXT_OK;
   e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) {
