@@ -8,9 +8,13 @@ same mask on every call, device and launch shape.
 ``rng`` holds (seed, offset): an int64 tensor on x's device, which a training step
 captured in a CUDA graph advances on the device (``rng[1] += 1``), or two Python
 integers.  The backward pass uses the values that the forward read, whatever has become
-of the tensor since.  ``layer`` is added to the seed, so the layers of a model take
-masks of their own from one ``rng``.  For Monte Carlo dropout at inference call it
-as in training.
+of the tensor since.  For Monte Carlo dropout at inference call it as in training.
+
+``layer`` is added to the seed, so the layers of a model take masks of their own from one
+``rng``.  Layer i + 1 under seed s therefore has the mask of layer i under seed s + 1:
+seeds that are to be independent (ranks of a data-parallel job, samples of Monte Carlo
+dropout) have to lie further apart than the layers do, as ``base + rank * 2**32`` does, or
+to differ in the offset.
 
 The rate is ``round(65536 p) / 65536``: one 16-bit random word decides about an
 element, and the scale is made from that rate.

@@ -34,7 +34,8 @@ def _pointwise(x: Tensor, conv: nn.Conv3d) -> Tensor:
 class ChannelMixer3d(nn.Module):
     """``forward(x, rng)``: x [N, C, D, H, W] in float32, bfloat16 or float16, ``rng`` the
     [seed, offset] tensor of :func:`dropout`, needed while training with ``p > 0``.  ``layer``
-    tells the mixers of one model apart in their masks.
+    tells the mixers of one model apart in their masks; seeds of independent models lie further
+    apart than their layers.
 
     The branch runs in x's type and the result has it.  Under autocast the convolutions of
     float32 or non-contiguous features, which are torch's, run in autocast's type."""

@@ -216,3 +216,10 @@ def test_words_match_numpy_layout():
         p = float(t) / 65536
         got = mx.dropout(torch.ones(16, device="cuda"), p, (7, 9)) != 0
         assert got.cpu().tolist() == (w >= t).tolist()
+
+
+def test_spaced_seeds_give_every_layer_a_mask_of_its_own():
+    """`layer` is added to the seed: seeds further apart than the layers, as the function's notes ask, share no mask."""
+    x = torch.ones(4096, device="cuda")
+    masks = [mx.dropout(x, 0.5, (7 + rank * 2**32, 0), layer=layer) != 0 for rank in range(4) for layer in range(4)]
+    assert len({tuple(m.cpu().tolist()) for m in masks}) == 16
