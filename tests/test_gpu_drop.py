@@ -223,3 +223,18 @@ def test_spaced_seeds_give_every_layer_a_mask_of_its_own():
     x = torch.ones(4096, device="cuda")
     masks = [mx.dropout(x, 0.5, (7 + rank * 2**32, 0), layer=layer) != 0 for rank in range(4) for layer in range(4)]
     assert len({tuple(m.cpu().tolist()) for m in masks}) == 16
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_masks_with_residual_and_gradients(dtype):
+    """Enough elements for several groups per thread in every type, the last CTA's ragged; the whole mask exactly."""
+    n, p = 10_000_005, 0.1
+    x, r, dy = data(n, dtype)
+    keep = kept(n, p, 31, 2**33 + 5)
+    xg, rg = x.clone().requires_grad_(), r.clone().requires_grad_()
+    y = mx.dropout(xg, p, torch.tensor([30, 2**33 + 5], device="cuda"), residual=rg, layer=1)
+    assert torch.equal(y, want(x, keep, p, r))
+    dx, dr = torch.autograd.grad(y, (xg, rg), dy)
+    assert torch.equal(dx, want(dy, keep, p)) and torch.equal(dr, dy)
+    assert torch.equal(mx.dropout(x, p, (31, 2**33 + 5)), want(x, keep, p))
+    assert nat.device_error() == 0

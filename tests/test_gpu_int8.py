@@ -408,3 +408,20 @@ def test_a_cast_module_keeps_its_numbers(cast):
     assert torch.equal(model(x), want)
     without = cast(mx.Int8Pointwise3d(torch.nn.Conv3d(24, 40, 1, bias=False).cuda()))
     assert without.bias is None and without(x).shape == want.shape
+
+
+UNSTAGED = [((2, 64, 33 * 35 * 37), 100, 1), ((1, 64, 33 * 35 * 37), 512, 1), ((1, 32, 33 * 35 * 37), 64, 1),
+            ((1, 512, 33 * 35 * 37), 128, 1), ((100003, 64), 77, -1), ((70001, 130), 301, -1)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape,n,dim", UNSTAGED)
+def test_many_tiles_off_16_byte_rows(shape, n, dim, dtype):
+    """Odd patches and odd widths: several tiles on each SM, so that accumulators are used again (two
+    of 256 columns, four of up to 128), and a ragged last tile of tokens and of channels."""
+    k = shape[dim]
+    w, s, b = weights(n, k, seed=n)
+    x = activations(shape, dtype, seed=k)
+    y = check(x, w, s, b, dim)
+    first = x[:1] if dim == 1 else x[:37]  # the bits do not depend on the company
+    assert torch.equal(mx.int8_linear(first, w, s, b, dim=dim), y[: first.shape[0]])

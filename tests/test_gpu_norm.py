@@ -391,3 +391,15 @@ def test_the_fold_reads_the_partials_of_its_own_call(shape, dim):
     results = [check_free(x, w, b, gradients[i % 4], dim)[2:] for i in range(60)]  # queued, not waited for
     for i, got in enumerate(results):
         assert all(torch.equal(p, q) for p, q in zip(got, want[i % 4], strict=True)), i
+
+
+@pytest.mark.parametrize("rows,c,dtype", [
+    (60001, 24, torch.float32), (40009, 97, torch.float32), (30011, 100, torch.float32), (20011, 522, torch.float32),
+    (9001, 1000, torch.float32), (4001, 2047, torch.float32), (4003, 4096, torch.float32), (2003, 5000, torch.float32),
+    (40009, 98, torch.bfloat16), (30011, 250, torch.float16), (20011, 522, torch.bfloat16), (20011, 522, torch.float16),
+    (4001, 4094, torch.bfloat16), (9001, 1000, torch.float16), (2003, 4095, torch.bfloat16), (2003, 3001, torch.float32),
+])
+def test_many_rows_of_each_word_and_type(rows, c, dtype):
+    """Several rows in flight per group (from 12 CTAs' worth of rows on each SM) for every word that rows can be
+    read in: 16 bytes, 4 bytes of 16-bit data, single elements."""
+    check(*inputs((rows, c), 1, dtype, seed=rows + c), -1)
