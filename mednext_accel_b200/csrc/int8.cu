@@ -2083,7 +2083,8 @@ int launch_quantize(const void* xv, int8_t* q, float* scale, long long outer, in
   }
   constexpr int E = 16 / sizeof(T);
   const int vecs = (int)((pitch + E - 1) / E);
-  // the registers of a warp hold 16 vectors per lane
+  // the registers of a warp hold 16 vectors per lane: 2048 columns of fp32, 4096 of 16 bits (wider ones go by
+  // single elements: 8192 x 4096 fp32 58 us, bf16 here 21)
   if (K % E == 0 && (reinterpret_cast<uintptr_t>(xv) & 15) == 0 && pitch - K < 16 && vecs <= 512) {
     int G = 1;
     while (G < 32 && G < vecs) G *= 2;

@@ -120,8 +120,8 @@ def dropout(x: Tensor, p: float, rng: Tensor | tuple[int, int], residual: Tensor
     ``residual``; see the module's notes for ``rng`` and ``layer``.
 
     x: float32, bfloat16 or float16 on an sm_100 device; residual: x's shape and type.
-    A dropped element contributes 0 whatever x holds there.  Differentiable once in x
-    and residual."""
+    A dropped element contributes 0 whatever x holds there.  The result is contiguous;
+    tensors that are not are copied first.  Differentiable once in x and residual."""
     if not x.is_cuda:
         raise ValueError("dropout requires CUDA tensors")
     if x.dtype not in DTYPES:

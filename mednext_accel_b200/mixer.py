@@ -3,9 +3,10 @@ of each voxel, with layer norm in front and dropout behind it.
 
     y = x + dropout(project(gelu(expand(layer_norm(x)))))
 
-Training runs the layer norm, the tensor-core pointwise products of the block and the
-counter-based dropout, whose residual add is the branch's; :meth:`ChannelMixer3d.int8`
-gives the serving form, whose two products run in 8-bit integers.  No reference
+Training runs the layer norm, the tensor-core pointwise products of the block (16-bit
+contiguous features; others take torch's convolutions), torch's GELU and the counter-based
+dropout, whose residual add is the branch's; :meth:`ChannelMixer3d.int8` gives the serving
+form, whose two products run in 8-bit integers.  No reference
 counterpart: the reference's blocks normalise each channel over the volume and have no
 dropout.
 """
